@@ -3,7 +3,7 @@
   adamw        `adamw_step`: decoupled-decay Adam over a list of tensors at once, 32-bit moments, gradients optionally clipped by
                the norm of all of them together
   adamw8       `adamw8_step`: the same with both moments in 8 bits, blocks of 256 elements under a power of two each; the moments
-               come back as the values that they stand for (`adamw8_moments`; at most five significant bits: exact in bfloat16)
+               come back as the values that they stand for (`adamw8_moments`; at most four significant bits: exact in bfloat16)
   balance      `balance_loss`: softmax over the superpoints, how often each is among a point's K largest, and the loss
                M * sum(share of the choices * mean probability), with its gradient by the logits
   neighbours   `neighbour_balance`: the same loss on the neighbour weights of points that see K superpoints each
@@ -164,17 +164,18 @@ def prepare(case, seed):
             state["m"][k].copy_(m)
             state["v"][k].copy_(root * root)
         else:
-            state["states"].append(_encode(m, root, torch.full((n,), 0.5, device=DEVICE), torch.full((n,), 0.5, device=DEVICE)))
+            state["states"].append(_encode(m, root * root, torch.full((n,), 0.5, device=DEVICE), torch.full((n,), 0.5, device=DEVICE)))
     if case["clip"]:  # as in training: the clipped norm is a part of what the gradients have
         state["max_norm"] = 0.3 * float(flat["grad"].double().norm())
     return state
 
 
 # ---- the 8-bit moments --------------------------------------------------------------------------------------------------
-# One tensor of bytes: codes of m [blocks * 256], codes of r = sqrt(v) [blocks * 256], then (m, r) exponents [blocks, 2]. A
-# code's magnitude stands for u units: u itself below one binade of fractions, then (fractions + fraction) << (exponent - 1). The
-# unit is a power of two such that the block's largest value lies in the highest binade. m has a sign and 3 bits of fraction, r
-# 4. An exponent byte is that of the largest value as float32 has it: 0 for a block of zeros, 255 if a value is not finite.
+# One tensor of bytes: codes of m [blocks * 256], codes of v [blocks * 256], then (m, v) exponents [blocks, 2]. A code's
+# magnitude has 3 bits of fraction below 4 (m, with a sign above) or 5 (v) bits of exponent. It stands for u units: u itself below
+# one binade of fractions, then (8 + fraction) << (exponent - 1). The unit is a power of two such that the block's largest value
+# lies in the highest binade. An exponent byte is that of the largest value as float32 has it: 0 for a block of zeros, 255 if a
+# value is not finite. v > 0 stays > 0.
 
 
 def _mix(x):
@@ -185,7 +186,7 @@ def _mix(x):
 
 
 def _noise(n, step, seed):
-    """What is added before rounding down, for m and for r: 16 bits each of a hash of the element, the step and the seed."""
+    """What is added before rounding down, for m and for v: 16 bits each of a hash of the element, the step and the seed."""
     key = _mix((int(step) + seed * 0x9E3779B1) & 0xFFFFFFFF)
     h = _mix((torch.arange(n, device=DEVICE) * 0x9E3779B1 + key) & 0xFFFFFFFF)
     return (h & 0xFFFF).double() / 65536, (h >> 16).double() / 65536
@@ -196,40 +197,40 @@ def _blocks(x):
 
 
 def _codes(x, noise, bits):
-    """(codes [blocks, 256], exponent bytes [blocks]) of values >= 0, `bits` bits of fraction."""
+    """(codes [blocks, 256], exponent bytes [blocks]) of values >= 0, `bits` bits of exponent."""
     x, noise = _blocks(x), _blocks(noise)
     top = x.amax(dim=1)
     exponent = torch.frexp(top)[1].long() - 1
-    y = x.double() * torch.exp2((14 + bits - exponent).double())[:, None]
+    y = x.double() * torch.exp2(((1 << bits) + 1 - exponent).double())[:, None]  # in units
     # NaN and infinities are gone with the block; what is left of them here does not matter
     y = torch.nan_to_num(y, 0.0, 0.0, 0.0)
-    binade = torch.clamp(torch.frexp(y)[1].long() - 1, min=bits)
-    k = torch.floor(y * torch.exp2((bits - binade).double()) + noise.double()).long()
-    code = torch.clamp(k + ((binade - bits) << bits), max=(1 << (bits + 4)) - 1)
+    binade = torch.clamp(torch.frexp(y)[1].long() - 1, min=3)
+    k = torch.floor(y * torch.exp2((3 - binade).double()) + noise.double()).long()
+    code = torch.clamp(k + ((binade - 3) << 3), max=(8 << bits) - 1)
     scale = torch.where(torch.isfinite(top), torch.where(top > 0, torch.clamp(exponent + 127, 1, 254), 0), 255)
     return code, scale
 
 
-def _encode(m, root, noise_m, noise_r):
-    code, scale_m = _codes(m.abs(), noise_m, 3)
+def _encode(m, v, noise_m, noise_v):
+    code, scale_m = _codes(m.abs(), noise_m, 4)
     code_m = torch.where((_blocks(m) < 0) & (code > 0), code + 128, code)
-    code_r, scale_r = _codes(root, noise_r, 4)
-    code_r = torch.where((code_r == 0) & (_blocks(root) > 0), 1, code_r)
-    return torch.cat([code_m.view(-1), code_r.view(-1), torch.stack([scale_m, scale_r], dim=1).view(-1)]).to(torch.uint8)
+    code_v, scale_v = _codes(v, noise_v, 5)
+    code_v = torch.where((code_v == 0) & (_blocks(v) > 0), 1, code_v)
+    return torch.cat([code_m.view(-1), code_v.view(-1), torch.stack([scale_m, scale_v], dim=1).view(-1)]).to(torch.uint8)
 
 
 def _values(code, scale, bits):
-    units = torch.where(code < (1 << bits), code, ((1 << bits) + (code & ((1 << bits) - 1))) << torch.clamp((code >> bits) - 1, min=0))
-    value = units.double() * torch.exp2((scale - 127 - 14 - bits).double())[:, None]
+    units = torch.where(code < 8, code, (8 + (code & 7)) << torch.clamp((code >> 3) - 1, min=0))
+    value = units.double() * torch.exp2((scale - 128 - (1 << bits)).double())[:, None]
     return torch.where(scale[:, None] == 255, math.nan, value)
 
 
 def _decode(state, n):
-    """(m, r) of a state, float32."""
+    """(m, v) of a state, float32."""
     blocks = -(-n // BLOCK)
     codes, scales = state[:blocks * 512].long().view(2, blocks, BLOCK), state[blocks * 512:].long().view(blocks, 2)
-    m = _values(codes[0] & 127, scales[:, 0], 3) * torch.where(codes[0] > 127, -1, 1)
-    return m.view(-1)[:n].float(), _values(codes[1], scales[:, 1], 4).view(-1)[:n].float()
+    m = _values(codes[0] & 127, scales[:, 0], 4) * torch.where(codes[0] > 127, -1, 1)
+    return m.view(-1)[:n].float(), _values(codes[1], scales[:, 1], 5).view(-1)[:n].float()
 
 
 # ---- one pass, plain ------------------------------------------------------------------------------------------------------
@@ -259,9 +260,8 @@ def _plain_step(s):
             s["m"][k].copy_(m)
             s["v"][k].copy_(v)
         else:
-            m, r = _decode(s["states"][k], len(p))
-            new, m, v = _plain_update(p.float(), g, m, r * r, step, rate)
-            s["states"][k].copy_(_encode(m, torch.sqrt(v), *_noise(len(p), step, s["seed"])))
+            new, m, v = _plain_update(p.float(), g, *_decode(s["states"][k], len(p)), step, rate)
+            s["states"][k].copy_(_encode(m, v, *_noise(len(p), step, s["seed"])))
             moments.append([x.bfloat16() for x in _decode(s["states"][k], len(p))])
         p.copy_(new)
     return norm, moments
@@ -371,28 +371,28 @@ def _exact_hash(x):
     return x ^ (x >> 16)
 
 
-def _exact_round(x, noise, fractions):
-    """Values of x >= 0 as blocks of 256 keep them."""
+def _exact_round(x, noise, binades):
+    """Values of x >= 0 as blocks of 256 keep them, and what the smallest of their codes stands for."""
     n, blocks = len(x), (len(x) + 255) // 256
     padded = x.new_zeros(2, blocks * 256)
     padded[0, :n], padded[1, :n] = x, noise
     x, noise = padded.view(2, blocks, 256)
     top = torch.floor(torch.log2(x.amax(dim=1, keepdim=True).clamp(min=2.0 ** -126)))
-    smallest = top - 14  # of the exponents with a full fraction
+    smallest = top - binades + 2  # of the exponents with a full fraction
     exponent = torch.maximum(torch.floor(torch.log2(x.clamp(min=2.0 ** -300))), smallest)
-    spacing = 2.0 ** exponent / fractions
+    spacing = 2.0 ** exponent / 8
     kept = torch.floor(x / spacing + noise) * spacing
-    most = 2.0 ** top * (2 - 1 / fractions)
-    return torch.minimum(kept, most).view(-1)[:n], (2.0 ** smallest / fractions).expand(-1, 256).reshape(-1)[:n]
+    most = 2.0 ** top * (2 - 1 / 8)
+    return torch.minimum(kept, most).view(-1)[:n], (2.0 ** smallest / 8).expand(-1, 256).reshape(-1)[:n]
 
 
 def _exact_moments(state):
-    """m and r of a state from its bytes, by tables of the 128 and 256 magnitudes."""
+    """m and v of a state from its bytes, by tables of the 128 and 256 magnitudes."""
     blocks = len(state) // 514
     tables = []
-    for fractions in (8, 16):
-        tables.append(torch.tensor([f if e == 0 else (fractions + f) * 2.0 ** (e - 1) for e in range(16) for f in range(fractions)],
-                                   dtype=torch.float64, device=DEVICE) / (fractions * 2.0 ** 14))
+    for binades in (16, 32):
+        tables.append(torch.tensor([f if e == 0 else (8 + f) * 2.0 ** (e - 1) for e in range(binades) for f in range(8)],
+                                   dtype=torch.float64, device=DEVICE) / (8 * 2.0 ** (binades - 2)))
     scale = 2.0 ** (state[512 * blocks:].double().view(blocks, 2) - 127)
     first, second = state[:256 * blocks].view(blocks, 256).long(), state[256 * blocks:512 * blocks].view(blocks, 256).long()
     m = tables[0][first % 128] * (1 - 2 * (first // 128)) * scale[:, :1]
@@ -403,15 +403,14 @@ def _exact_step(case, s):
     grads = [g.double() for g in s["grad"]]
     norm = torch.sqrt(torch.stack([torch.dot(g, g) for g in grads]).sum())
     clip = 1.0 if s["max_norm"] is None else min(1.0, s["max_norm"] / (float(norm) + 1e-6))
-    param, first, second, moments = (torch.zeros_like(s["flat"]["param"], dtype=torch.float64) for _ in range(3)), None, None, []
-    param, first, second = param
+    param, first, second = (torch.zeros_like(s["flat"]["param"], dtype=torch.float64) for _ in range(3))
+    moments = []
     for k, g in enumerate(grads):
         g, t, n, rate = g * clip, float(s["steps"][k]) + 1, len(g), s["rates"][k]
         if case["kind"] == "adamw":
             m, v = s["m"][k].double(), s["v"][k].double()
         else:
-            m, r = _exact_moments(s["states"][k])
-            m, v = m[:n], r[:n] ** 2
+            m, v = (x[:n] for x in _exact_moments(s["states"][k]))
         m, v = m + (g - m) * (1 - BETAS[0]), v + (g * g - v) * (1 - BETAS[1])
         m_hat, v_hat = m / (1 - BETAS[0] ** t), v / (1 - BETAS[1] ** t)
         x = s["param"][k].double()
@@ -422,10 +421,9 @@ def _exact_step(case, s):
         else:
             key = _exact_hash((int(t) + s["seed"] * 0x9E3779B1) % (1 << 32))
             h = _exact_hash((torch.arange(n, device=DEVICE, dtype=torch.int64) * 0x9E3779B1 + key) % (1 << 32))
-            r = v.sqrt()
-            kept_m, _ = _exact_round(m.abs(), (h % 65536) / 65536.0, 8)
-            kept_r, unit = _exact_round(r, (h // 65536) / 65536.0, 16)
-            moments.append([torch.sign(m) * kept_m, torch.where((kept_r == 0) & (r > 0), unit, kept_r)])
+            kept_m, _ = _exact_round(m.abs(), (h % 65536) / 65536.0, 16)
+            kept_v, unit = _exact_round(v, (h // 65536) / 65536.0, 32)
+            moments.append([torch.sign(m) * kept_m, torch.where((kept_v == 0) & (v > 0), unit, kept_v)])
     out = {"param": param, "norm": norm if s["max_norm"] is not None else None}
     out.update({"m": first, "v": second} if case["kind"] == "adamw" else {"moments": moments})
     return out
