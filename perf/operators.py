@@ -173,9 +173,9 @@ def prepare(case, seed):
 # ---- the 8-bit moments --------------------------------------------------------------------------------------------------
 # One tensor of bytes: codes of m [blocks * 256], codes of v [blocks * 256], then (m, v) exponents [blocks, 2]. A code's
 # magnitude has 3 bits of fraction below 4 (m, with a sign above) or 5 (v) bits of exponent. It stands for u units: u itself below
-# one binade of fractions, then (8 + fraction) << (exponent - 1). The unit is a power of two such that the block's largest value
-# lies in the highest binade. An exponent byte is that of the largest value as float32 has it: 0 for a block of zeros, 255 if a
-# value is not finite. v > 0 stays > 0.
+# one binade of fractions, then (8 + fraction) << (exponent - 1). The unit is the smallest power of two for which the block's
+# largest value is no larger than the highest code's. An exponent byte is that of the highest binade as float32 has it: 0 for a
+# block of zeros, 255 if a value is not finite. v > 0 stays > 0.
 
 
 def _mix(x):
@@ -200,7 +200,8 @@ def _codes(x, noise, bits):
     """(codes [blocks, 256], exponent bytes [blocks]) of values >= 0, `bits` bits of exponent."""
     x, noise = _blocks(x), _blocks(noise)
     top = x.amax(dim=1)
-    exponent = torch.frexp(top)[1].long() - 1
+    fraction, exponent = torch.frexp(top)  # fraction in [0.5, 1)
+    exponent = exponent.long() - 1 + (fraction > 1.875 / 2)
     y = x.double() * torch.exp2(((1 << bits) + 1 - exponent).double())[:, None]  # in units
     # NaN and infinities are gone with the block; what is left of them here does not matter
     y = torch.nan_to_num(y, 0.0, 0.0, 0.0)
@@ -377,7 +378,9 @@ def _exact_round(x, noise, binades):
     padded = x.new_zeros(2, blocks * 256)
     padded[0, :n], padded[1, :n] = x, noise
     x, noise = padded.view(2, blocks, 256)
-    top = torch.floor(torch.log2(x.amax(dim=1, keepdim=True).clamp(min=2.0 ** -126)))
+    largest = x.amax(dim=1, keepdim=True).clamp(min=2.0 ** -126)
+    top = torch.floor(torch.log2(largest))
+    top = top + (largest > 1.875 * 2.0 ** top)
     smallest = top - binades + 2  # of the exponents with a full fraction
     exponent = torch.maximum(torch.floor(torch.log2(x.clamp(min=2.0 ** -300))), smallest)
     spacing = 2.0 ** exponent / 8
