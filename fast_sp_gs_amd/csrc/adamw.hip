@@ -1,0 +1,522 @@
+// AdamW (Adam with decoupled weight decay) over many tensors in one launch, moments in 32 bits or in 8, and what comes before it in a
+// step: the norm of all gradients together, by which they are clipped, and the corrections of step counts kept on the device.
+//
+//   m = b1 m + (1 - b1) c g,  v = b2 v + (1 - b2) (c g)^2,  p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// with c = min(1, max_norm / (|g| + 1e-6)) where a norm is given. Every tensor has its own rates and step count. Parameters and gradients
+// are float32, float16 or bfloat16 (rounded to nearest once, when they are stored); the moments are float32 or the 8-bit blocks below.
+//
+// Moments in 8 bits. Adam's moments move by parts in ten (m) and in a thousand (v) of a step, far less than the spacing of 8-bit
+// values: rounding to the nearest one would leave them where they are for good. They are rounded down after a number in [0, 1) spacings
+// has been added, 16 bits of a hash of (element, step count, seed), so that the mean of what is kept is the value (of v itself: rounding
+// its root in that way would raise the mean of v by the variance of the root). A block is 256 consecutive elements, four for each lane of
+// a wavefront, under one power of two for each moment, the smallest for which the highest code is not below the largest value (a
+// value above it could only be rounded down).
+//   m  sign, 4 bits of exponent, 3 of fraction: 18 binades
+//   v  5 bits of exponent, 3 of fraction: 34 binades, 17 of the root; a value above 0 is kept above 0, since an element whose
+//      second moment vanished before its first would be divided by eps alone
+// Both are the top of a float32 with a small exponent: decoding shifts the code to that place and scales by a power of two, encoding
+// scales, adds the noise below the last kept bit and shifts, subnormal values of the format included, with no case of its own.
+// A state is one allocation: codes of m [256 b], codes of v [256 b], exponents (m, v) [b][2] for b blocks. Exponents are those of
+// float32 (biased by 127); 0 is a block of zeros, 255 one that held an infinity or a NaN, all of whose values read as NaN.
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+#include <cmath>
+
+#include "../../include/fsgs.h"
+#include "common.hpp"
+
+namespace fsgs {
+namespace {
+
+constexpr int kBlock = 256;        // elements of an 8-bit block
+constexpr int kMaxTensors = 48;    // a launch's table is passed by value: 80 bytes a tensor of the 4 KB that arguments may have
+constexpr int kNormBlocks = 1024;  // of the sum of squares: a sum each
+constexpr int kNormChunk = 8192;   // elements that a block sums before it looks for its next ones
+
+struct Rates {  // of one tensor's step, formed on the host or by adamw_rates_kernel
+  float step_size, inv_root_c2;
+  uint32_t key;  // of the step's noise
+  uint32_t pad;
+};
+
+struct AdamwTable {
+  void* param[kMaxTensors];
+  const void* grad[kMaxTensors];
+  void* m[kMaxTensors];  // 8-bit moments: the state
+  float* v[kMaxTensors];
+  int64_t count[kMaxTensors];
+  Rates rates[kMaxTensors];
+  float keep[kMaxTensors];  // 1 - lr wd
+  float eps[kMaxTensors];
+  unsigned first_block[kMaxTensors + 1];
+  int n;
+};
+static_assert(sizeof(AdamwTable) <= 4032, "kernel arguments");
+
+// The tensor that block `b` of a launch works on.
+__device__ __forceinline__ int tensor_of(const unsigned* first, int n, unsigned b) {
+  int low = 0, high = n;  // first[low] <= b < first[high]
+  while (high - low > 1) {
+    const int mid = (low + high) >> 1;
+    if (b >= first[mid]) low = mid;
+    else high = mid;
+  }
+  return low;
+}
+
+// ---- four elements at a time --------------------------------------------------------------------------------------------------
+template <typename T>
+struct alignas(4 * sizeof(T)) Four {
+  T x[4];
+};
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_float(__hip_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half(x); }
+template <>
+__device__ __forceinline__ __hip_bfloat16 from_float<__hip_bfloat16>(float x) { return __float2bfloat16(x); }
+
+// `left` elements are there; `whole`: all four, and their address allows one access.
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, int64_t left, bool whole, float out[4]) {
+  if (whole) {
+    const Four<T> q = *(const Four<T>*) p;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) out[k] = to_float(q.x[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) out[k] = k < left ? to_float(p[k]) : 0.0f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, int64_t left, bool whole, const float in[4]) {
+  if (whole) {
+    Four<T> q;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) q.x[k] = from_float<T>(in[k]);
+    *(Four<T>*) p = q;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < left) p[k] = from_float<T>(in[k]);
+  }
+}
+
+struct Step {
+  float b1, b2, c1, c2;  // c = 1 - b
+};
+
+// One element; the moments are replaced. Every operation rounds by itself, as a chain of tensor operations does.
+__device__ __forceinline__ float updated(const Step& s, const Rates& r, float keep, float eps, float p, float g, float& m, float& v) {
+#pragma clang fp contract(off)
+  m = s.b1 * m + s.c1 * g;
+  v = s.b2 * v + s.c2 * g * g;
+  return p * keep - r.step_size * m / (sqrtf(v) * r.inv_root_c2 + eps);
+}
+
+// ---- 32-bit moments -------------------------------------------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(256) adamw_kernel(AdamwTable t, Step s, const float* __restrict__ factor,
+                                                    const Rates* __restrict__ rates) {
+  const int q = tensor_of(t.first_block, t.n, blockIdx.x);
+  const int64_t e = (int64_t) (blockIdx.x - t.first_block[q]) * 1024 + threadIdx.x * 4, left = t.count[q] - e;
+  if (left <= 0) return;
+  const Rates r = rates ? rates[q] : t.rates[q];
+  const float c = factor ? factor[1] : 1.0f, keep = t.keep[q], eps = t.eps[q];
+  T* param = (T*) t.param[q] + e;
+  const T* grad = (const T*) t.grad[q] + e;
+  float *first = (float*) t.m[q] + e, *second = t.v[q] + e;
+  const bool whole = left >= 4 && (((uintptr_t) first | (uintptr_t) second) & 15) == 0 &&
+                     (((uintptr_t) param | (uintptr_t) grad) & (4 * sizeof(T) - 1)) == 0;
+  float p[4], g[4], m[4], v[4];
+  load4(param, left, whole, p), load4(grad, left, whole, g);
+  load4<float>(first, left, whole, m), load4<float>(second, left, whole, v);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) p[k] = updated(s, r, keep, eps, p[k], c * g[k], m[k], v[k]);
+  store4(param, left, whole, p);
+  store4<float>(first, left, whole, m), store4<float>(second, left, whole, v);
+}
+
+// ---- 8-bit moments ----------------------------------------------------------------------------------------------------------------
+__host__ __device__ __forceinline__ uint32_t mixed(uint32_t x) {
+  x = (x ^ (x >> 16)) * 0xBB67AE85u;
+  x = (x ^ (x >> 15)) * 0x3C6EF373u;
+  return x ^ (x >> 16);
+}
+constexpr uint32_t kStride = 0x9E3779B1u;  // between the hashes' arguments of neighbouring elements, and of seeds
+__host__ __device__ __forceinline__ uint32_t noise_key(uint32_t step, uint32_t seed) { return mixed(step + seed * kStride); }
+
+// Largest of a value over the wavefront's lanes, in scalar registers: four rotations within rows of 16 lanes, then the rows.
+template <int kCtrl>
+__device__ __forceinline__ uint32_t max_step(uint32_t x) {
+  return max(x, (uint32_t) __builtin_amdgcn_update_dpp(0, (int) x, kCtrl, 0xf, 0xf, true));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+  x = max_step<0x128>(x), x = max_step<0x124>(x), x = max_step<0x122>(x), x = max_step<0x121>(x);  // row_ror:8, 4, 2, 1
+  const uint32_t a = __builtin_amdgcn_readlane(x, 0), b = __builtin_amdgcn_readlane(x, 16);
+  const uint32_t c = __builtin_amdgcn_readlane(x, 32), d = __builtin_amdgcn_readlane(x, 48);
+  return max(max(a, b), max(c, d));
+}
+
+// From a code's place in a float32 (exponent 1 is its lowest binade) to that of its block, whose highest one is 2^kBits - 1.
+template <int kBits>  // of exponent
+__device__ __forceinline__ float decoded(uint32_t code, int exponent) {
+  const float x = ldexpf(__builtin_bit_cast(float, code << 20), exponent + 1 - (1 << kBits));
+  return exponent == 255 ? __builtin_nanf("") : x;
+}
+template <int kBits>
+__device__ __forceinline__ uint32_t encoded(float x, int exponent, uint32_t noise16) {
+  const uint32_t y = __builtin_bit_cast(uint32_t, ldexpf(x, (1 << kBits) - 1 - exponent));
+  return min((y + (noise16 << 4)) >> 20, (8u << kBits) - 1);
+}
+// A block's exponent byte from the bits of its largest magnitude (a NaN is larger than any): that of the next binade where the value is
+// above 1.875 of its own. Below the normal numbers the lowest normal exponent stands for all; 254 is the last of finite values.
+__device__ __forceinline__ int block_exponent(uint32_t top) {
+  if (top >= 0x7f800000u) return 255;
+  return top ? min(max((int) ((top + 0xfffffu) >> 23), 1), 254) : 0;
+}
+
+// Codes of four elements of a block, and the block's exponents; the noise of m in the low half of a word, of v in the high one.
+__device__ __forceinline__ void encode4(const float m[4], const float v[4], const uint32_t noise[4], uint32_t& codes_m,
+                                        uint32_t& codes_v, int& exponent_m, int& exponent_v) {
+  uint32_t top_m = 0, top_v = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    top_m = max(top_m, __builtin_bit_cast(uint32_t, m[k]) & 0x7fffffffu);
+    top_v = max(top_v, __builtin_bit_cast(uint32_t, v[k]) & 0x7fffffffu);
+  }
+  exponent_m = block_exponent(wave_max(top_m)), exponent_v = block_exponent(wave_max(top_v));
+  codes_m = codes_v = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t a = encoded<4>(fabsf(m[k]), exponent_m, noise[k] & 0xffffu);
+    uint32_t b = encoded<5>(v[k], exponent_v, noise[k] >> 16);
+    if (b == 0 && v[k] > 0.0f) b = 1;
+    codes_m |= (a | (m[k] < 0.0f && a ? 128u : 0u)) << (8 * k);
+    codes_v |= b << (8 * k);
+  }
+}
+
+struct StateView {  // of a tensor's 8-bit moments
+  uint8_t *m, *v, *exponents;
+};
+__host__ __device__ __forceinline__ StateView view_state(void* state, int64_t count) {
+  const int64_t b = (count + kBlock - 1) / kBlock;
+  uint8_t* at = (uint8_t*) state;
+  return {at, at + b * kBlock, at + 2 * b * kBlock};
+}
+
+__device__ __forceinline__ void decode(uint32_t a, uint32_t b, int exponent_m, int exponent_v, float& m, float& v) {
+  m = decoded<4>(a & 127, exponent_m), v = decoded<5>(b & 255, exponent_v);
+  if (a & 128) m = -m;
+}
+
+// A wavefront steps a block: a lane has four elements of it.
+template <typename T>
+__global__ void __launch_bounds__(256) adamw8_kernel(AdamwTable t, Step s, const float* __restrict__ factor,
+                                                     const Rates* __restrict__ rates) {
+  const int q = tensor_of(t.first_block, t.n, blockIdx.x);
+  const int64_t block = (int64_t) (blockIdx.x - t.first_block[q]) * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (block * kBlock >= t.count[q]) return;  // the whole wavefront
+  const int64_t e = block * kBlock + lane * 4, left = t.count[q] - e;
+  const Rates rate = rates ? rates[q] : t.rates[q];
+  const float c = factor ? factor[1] : 1.0f, keep = t.keep[q], eps = t.eps[q];
+  T* param = (T*) t.param[q] + e;
+  const T* grad = (const T*) t.grad[q] + e;
+  const StateView state = view_state(t.m[q], t.count[q]);
+  const bool whole = left >= 4 && (((uintptr_t) param | (uintptr_t) grad) & (4 * sizeof(T) - 1)) == 0;
+  float p[4], g[4], m[4], v[4];
+  load4(param, left, whole, p), load4(grad, left, whole, g);
+  const uint32_t old_m = *(const uint32_t*) (state.m + e), old_v = *(const uint32_t*) (state.v + e);
+  int exponent_m = state.exponents[2 * block], exponent_v = state.exponents[2 * block + 1];
+  uint32_t noise[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    decode(old_m >> (8 * k), old_v >> (8 * k), exponent_m, exponent_v, m[k], v[k]);
+    p[k] = updated(s, rate, keep, eps, p[k], c * g[k], m[k], v[k]);
+    if (k >= left) m[k] = v[k] = 0.0f;
+    noise[k] = mixed((uint32_t) (e + k) * kStride + rate.key);
+  }
+  uint32_t codes_m, codes_v;
+  encode4(m, v, noise, codes_m, codes_v, exponent_m, exponent_v);
+  store4(param, left, whole, p);
+  *(uint32_t*) (state.m + e) = codes_m, *(uint32_t*) (state.v + e) = codes_v;
+  if (lane == 0) *(uint16_t*) (state.exponents + 2 * block) = (uint16_t) (exponent_m | exponent_v << 8);
+}
+
+struct MomentsTable {
+  void* state[kMaxTensors];
+  void* m[kMaxTensors];
+  void* v[kMaxTensors];
+  int64_t count[kMaxTensors];
+  unsigned first_block[kMaxTensors + 1];
+  int n;
+};
+
+// The values that 8-bit moments stand for.
+template <typename T>
+__global__ void __launch_bounds__(256) adamw8_unpack_kernel(MomentsTable t) {
+  const int q = tensor_of(t.first_block, t.n, blockIdx.x);
+  const int64_t e = (int64_t) (blockIdx.x - t.first_block[q]) * 1024 + threadIdx.x * 4, left = t.count[q] - e;
+  if (left <= 0) return;
+  const StateView state = view_state(t.state[q], t.count[q]);
+  T *first = (T*) t.m[q] + e, *second = (T*) t.v[q] + e;
+  const bool whole = left >= 4 && (((uintptr_t) first | (uintptr_t) second) & (4 * sizeof(T) - 1)) == 0;
+  const uint32_t codes_m = *(const uint32_t*) (state.m + e), codes_v = *(const uint32_t*) (state.v + e);
+  const int exponent_m = state.exponents[2 * (e / kBlock)], exponent_v = state.exponents[2 * (e / kBlock) + 1];
+  float m[4], v[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) decode(codes_m >> (8 * k), codes_v >> (8 * k), exponent_m, exponent_v, m[k], v[k]);
+  store4(first, left, whole, m), store4(second, left, whole, v);
+}
+
+// 8-bit moments of given values (m, v), rounded to the nearest: they are taken over once, not step after step.
+__global__ void __launch_bounds__(256) adamw8_pack_kernel(MomentsTable t) {
+  const int q = tensor_of(t.first_block, t.n, blockIdx.x);
+  const int64_t block = (int64_t) (blockIdx.x - t.first_block[q]) * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (block * kBlock >= t.count[q]) return;
+  const int64_t e = block * kBlock + lane * 4, left = t.count[q] - e;
+  const StateView state = view_state(t.state[q], t.count[q]);
+  float m[4], v[4];
+  load4((const float*) t.m[q] + e, left, false, m), load4((const float*) t.v[q] + e, left, false, v);
+  const uint32_t noise[4] = {0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
+  uint32_t codes_m, codes_v;
+  int exponent_m, exponent_v;
+  encode4(m, v, noise, codes_m, codes_v, exponent_m, exponent_v);
+  *(uint32_t*) (state.m + e) = codes_m, *(uint32_t*) (state.v + e) = codes_v;
+  if (lane == 0) *(uint16_t*) (state.exponents + 2 * block) = (uint16_t) (exponent_m | exponent_v << 8);
+}
+
+// ---- the norm of all gradients --------------------------------------------------------------------------------------------------
+struct NormTable {
+  const void* grad[kMaxTensors];
+  int64_t count[kMaxTensors];
+  unsigned first_chunk[kMaxTensors + 1];
+  int n;
+};
+
+// Sum over the block's 256 threads, in a fixed order; valid in thread 0.
+__device__ __forceinline__ double block_sum(double x, double* s_wave) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) x += __shfl_down(x, d);
+  if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x >> 6] = x;
+  __syncthreads();
+  return ((s_wave[0] + s_wave[1]) + s_wave[2]) + s_wave[3];
+}
+
+// Sums of squares: a lane's 32 elements of a chunk in float32 (four sums of eight), everything above in float64.
+template <typename T>
+__global__ void __launch_bounds__(256) square_sums_kernel(NormTable t, double* __restrict__ sums) {
+  __shared__ double s_wave[4];
+  double total = 0.0;
+  for (unsigned chunk = blockIdx.x; chunk < t.first_chunk[t.n]; chunk += gridDim.x) {
+    const int q = tensor_of(t.first_chunk, t.n, chunk);
+    const int64_t at = (int64_t) (chunk - t.first_chunk[q]) * kNormChunk + threadIdx.x * 4, count = t.count[q];
+    const T* grad = (const T*) t.grad[q];
+    const bool aligned = ((uintptr_t) grad & (4 * sizeof(T) - 1)) == 0;
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < kNormChunk / 1024; ++j) {
+      const int64_t e = at + j * 1024;
+      if (e >= count) break;
+      float g[4];
+      load4(grad + e, count - e, aligned && count - e >= 4, g);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sum[k] = fmaf(g[k], g[k], sum[k]);
+    }
+    total += ((double) sum[0] + sum[1]) + ((double) sum[2] + sum[3]);
+  }
+  total = block_sum(total, s_wave);
+  if (threadIdx.x == 0) sums[blockIdx.x] = total;
+}
+
+__global__ void __launch_bounds__(256) norm_factor_kernel(int n, const double* __restrict__ sums, double max_norm,
+                                                          float* __restrict__ out) {
+  __shared__ double s_wave[4];
+  double total = 0.0;
+  for (int k = threadIdx.x; k < n; k += 256) total += sums[k];
+  total = block_sum(total, s_wave);
+  if (threadIdx.x != 0) return;
+  const float norm = (float) sqrt(total);
+  const float factor = (float) max_norm / (norm + 1e-6f);
+  // a NaN passes, as a comparison with it would not let it
+  out[0] = norm, out[1] = factor > 1.0f ? 1.0f : factor;
+}
+
+// ---- step counts on the device ------------------------------------------------------------------------------------------------
+struct StepTable {
+  float* step[kMaxTensors];
+  double lr[kMaxTensors];
+  int n;
+};
+__global__ void __launch_bounds__(64) adamw_rates_kernel(StepTable t, double b1, double b2, uint32_t seed, Rates* __restrict__ rates) {
+  const int q = threadIdx.x;
+  if (q >= t.n) return;
+  const float step = *t.step[q] + 1.0f;
+  *t.step[q] = step;
+  Rates r{};
+  r.step_size   = (float) (t.lr[q] / (1.0 - pow(b1, (double) step)));
+  r.inv_root_c2 = (float) (1.0 / sqrt(1.0 - pow(b2, (double) step)));
+  r.key         = noise_key((uint32_t) step, seed);
+  rates[q] = r;
+}
+
+enum Type { kFloat32 = FSGS_DTYPE_F32, kFloat16 = FSGS_DTYPE_F16, kBfloat16 = FSGS_DTYPE_BF16 };
+size_t type_size(int type) { return type == kFloat32 ? 4 : 2; }
+bool is_type(int type) { return type == kFloat32 || type == kFloat16 || type == kBfloat16; }
+
+// first[q]: blocks before tensor q at `per_block` elements a block
+template <typename Table>
+int lay_out(const char* what, Table& t, unsigned* first, int n, const int64_t* count, int64_t per_block) {
+  int64_t blocks = 0;
+  for (int q = 0; q < n; ++q) {
+    FSGS_REQUIRE(count[q] >= 0, "%s: bad tensor %d", what, q);
+    t.count[q] = count[q], first[q] = (unsigned) blocks;
+    blocks += (count[q] + per_block - 1) / per_block;
+    FSGS_REQUIRE(blocks < (int64_t) 0x7fffffff, "%s: too many elements", what);
+  }
+  first[n] = (unsigned) blocks;
+  t.n = n;
+  return kOk;
+}
+
+}  // namespace
+}  // namespace fsgs
+
+using namespace fsgs;
+
+FSGS_API int fsgs_adamw_max_tensors(void) { return kMaxTensors; }
+FSGS_API size_t fsgs_adamw8_state_bytes(int64_t count) {
+  return count <= 0 ? 0 : (size_t) ((count + kBlock - 1) / kBlock) * (2 * kBlock + 2);
+}
+FSGS_API int fsgs_grad_square_sums_max(void) { return kNormBlocks; }
+FSGS_API size_t fsgs_adamw_rates_bytes(int n_tensors) { return (size_t) (n_tensors > 0 ? n_tensors : 0) * sizeof(Rates); }
+
+FSGS_API int fsgs_grad_square_sums(int n_tensors, int dtype, const int64_t* count, const void* const* grad, int n_sums, double* sums,
+                                   void* stream) {
+  const char* what = "grad_norm";
+  FSGS_REQUIRE(n_tensors > 0 && n_tensors <= kMaxTensors && is_type(dtype) && n_sums > 0 && n_sums <= kNormBlocks,
+               "%s: bad arguments (at most %d tensors)", what, kMaxTensors);
+  FSGS_REQUIRE(count && grad && sums, "%s: null pointer", what);
+  NormTable t{};
+  if (const int rc = lay_out(what, t, t.first_chunk, n_tensors, count, kNormChunk)) return rc;
+  for (int q = 0; q < n_tensors; ++q) {
+    FSGS_REQUIRE(count[q] == 0 || (grad[q] && (uintptr_t) grad[q] % type_size(dtype) == 0), "%s: bad tensor %d", what, q);
+    t.grad[q] = grad[q];
+  }
+  auto kernel = dtype == kFloat32 ? square_sums_kernel<float> : dtype == kFloat16 ? square_sums_kernel<__half> : square_sums_kernel<__hip_bfloat16>;
+  hipLaunchKernelGGL(kernel, dim3(n_sums), dim3(256), 0, (hipStream_t) stream, t, sums);
+  return check_launch(what);
+}
+
+FSGS_API int fsgs_grad_norm_factor(int n_sums, const double* sums, double max_norm, float* norm_and_factor, void* stream) {
+  FSGS_REQUIRE(n_sums >= 0 && (n_sums == 0 || sums) && norm_and_factor, "grad_norm: null pointer");
+  hipLaunchKernelGGL(norm_factor_kernel, dim3(1), dim3(256), 0, (hipStream_t) stream, n_sums, sums, max_norm, norm_and_factor);
+  return check_launch("grad_norm");
+}
+
+FSGS_API int fsgs_adamw_rates(int n_tensors, float* const* step, const double* lr, double b1, double b2, uint32_t seed, void* rates,
+                              void* stream) {
+  const char* what = "adamw";
+  FSGS_REQUIRE(n_tensors >= 0 && n_tensors <= kMaxTensors, "%s: at most %d tensors", what, kMaxTensors);
+  if (n_tensors == 0) return kOk;
+  FSGS_REQUIRE(step && lr && rates && ((uintptr_t) rates & 15) == 0, "%s: null pointer", what);
+  StepTable t{};
+  t.n = n_tensors;
+  for (int q = 0; q < n_tensors; ++q) {
+    FSGS_REQUIRE(step[q], "%s: bad tensor %d", what, q);
+    t.step[q] = step[q], t.lr[q] = lr[q];
+  }
+  hipLaunchKernelGGL(adamw_rates_kernel, dim3(1), dim3(64), 0, (hipStream_t) stream, t, b1, b2, seed, (Rates*) rates);
+  return check_launch(what);
+}
+
+namespace {
+int adamw_update(const char* what, int bits, int n, int dtype, const int64_t* count, const double* step, const double* lr, double b1,
+                 double b2, const double* eps, const double* decay, uint32_t seed, const void* rates, const float* factor,
+                 void* const* param, const void* const* grad, void* const* m, float* const* v, void* stream) {
+  FSGS_REQUIRE(n >= 0 && n <= kMaxTensors && is_type(dtype), "%s: bad arguments (at most %d tensors)", what, kMaxTensors);
+  if (n == 0) return kOk;
+  FSGS_REQUIRE(count && lr && eps && decay && param && grad && m && (v || bits == 8) && (step || rates), "%s: null pointer", what);
+  AdamwTable t{};
+  if (const int rc = lay_out(what, t, t.first_block, n, count, 1024)) return rc;
+  if (t.first_block[n] == 0) return kOk;
+  for (int q = 0; q < n; ++q) {
+    const uintptr_t wide = (uintptr_t) m[q] | (v ? (uintptr_t) v[q] : 0), narrow = (uintptr_t) param[q] | (uintptr_t) grad[q];
+    FSGS_REQUIRE(count[q] == 0 || (param[q] && grad[q] && m[q] && (!v || v[q]) && wide % 4 == 0 && narrow % type_size(dtype) == 0),
+                 "%s: bad tensor %d", what, q);
+    t.param[q] = param[q], t.grad[q] = grad[q], t.m[q] = m[q], t.v[q] = v ? v[q] : nullptr;
+    t.keep[q] = (float) (1.0 - lr[q] * decay[q]), t.eps[q] = (float) eps[q];
+    if (rates) continue;
+    FSGS_REQUIRE(step[q] >= 1.0, "%s: tensor %d has taken no step", what, q);
+    t.rates[q].step_size   = (float) (lr[q] / (1.0 - std::pow(b1, step[q])));
+    t.rates[q].inv_root_c2 = (float) (1.0 / std::sqrt(1.0 - std::pow(b2, step[q])));
+    t.rates[q].key         = noise_key((uint32_t) (int64_t) step[q], seed);
+  }
+  const Step s{(float) b1, (float) b2, (float) (1.0 - b1), (float) (1.0 - b2)};
+  auto kernel = bits == 8 ? (dtype == kFloat32 ? adamw8_kernel<float> : dtype == kFloat16 ? adamw8_kernel<__half> : adamw8_kernel<__hip_bfloat16>)
+                          : (dtype == kFloat32 ? adamw_kernel<float> : dtype == kFloat16 ? adamw_kernel<__half> : adamw_kernel<__hip_bfloat16>);
+  hipLaunchKernelGGL(kernel, dim3(t.first_block[n]), dim3(256), 0, (hipStream_t) stream, t, s, factor, (const Rates*) rates);
+  return check_launch(what);
+}
+
+int moments(const char* what, int n, const int64_t* count, const void* const* state, const void* const* m, const void* const* v,
+            size_t size, MomentsTable& t) {
+  FSGS_REQUIRE(n >= 0 && n <= kMaxTensors, "%s: at most %d tensors", what, kMaxTensors);
+  if (n == 0) return kOk;
+  FSGS_REQUIRE(count && state && m && v, "%s: null pointer", what);
+  if (const int rc = lay_out(what, t, t.first_block, n, count, 1024)) return rc;
+  for (int q = 0; q < n; ++q) {
+    FSGS_REQUIRE(count[q] == 0 || (state[q] && m[q] && v[q] && (uintptr_t) state[q] % 4 == 0 &&
+                                   ((uintptr_t) m[q] | (uintptr_t) v[q]) % size == 0), "%s: bad tensor %d", what, q);
+    t.state[q] = (void*) state[q], t.m[q] = (void*) m[q], t.v[q] = (void*) v[q];
+  }
+  return kOk;
+}
+}  // namespace
+
+FSGS_API int fsgs_adamw_update_multi(int n_tensors, int dtype, const int64_t* count, const double* step, const double* lr, double b1,
+    double b2, const double* eps, const double* decay, const void* rates, const float* norm_and_factor, void* const* param,
+    const void* const* grad, float* const* m, float* const* v, void* stream) {
+  FSGS_REQUIRE(n_tensors == 0 || v, "adamw: null pointer");
+  return adamw_update("adamw", 32, n_tensors, dtype, count, step, lr, b1, b2, eps, decay, 0, rates, norm_and_factor, param, grad,
+                      (void* const*) m, v, stream);
+}
+
+FSGS_API int fsgs_adamw8_update_multi(int n_tensors, int dtype, const int64_t* count, const double* step, const double* lr, double b1,
+    double b2, const double* eps, const double* decay, uint32_t seed, const void* rates, const float* norm_and_factor,
+    void* const* param, const void* const* grad, void* const* state, void* stream) {
+  return adamw_update("adamw8", 8, n_tensors, dtype, count, step, lr, b1, b2, eps, decay, seed, rates, norm_and_factor, param, grad,
+                      state, nullptr, stream);
+}
+
+FSGS_API int fsgs_adamw8_unpack_multi(int n_tensors, int dtype, const int64_t* count, const void* const* state, void* const* m,
+                                      void* const* v, void* stream) {
+  const char* what = "adamw8_moments";
+  FSGS_REQUIRE(is_type(dtype), "%s: element type not supported", what);
+  MomentsTable t{};
+  if (const int rc = moments(what, n_tensors, count, state, m, v, type_size(dtype), t)) return rc;
+  if (t.first_block[t.n] == 0) return kOk;
+  auto kernel = dtype == kFloat32 ? adamw8_unpack_kernel<float> : dtype == kFloat16 ? adamw8_unpack_kernel<__half> : adamw8_unpack_kernel<__hip_bfloat16>;
+  hipLaunchKernelGGL(kernel, dim3(t.first_block[t.n]), dim3(256), 0, (hipStream_t) stream, t);
+  return check_launch(what);
+}
+
+FSGS_API int fsgs_adamw8_pack_multi(int n_tensors, const int64_t* count, const float* const* m, const float* const* v,
+                                    void* const* state, void* stream) {
+  const char* what = "adamw8_pack";
+  MomentsTable t{};
+  if (const int rc = moments(what, n_tensors, count, state, (const void* const*) m, (const void* const*) v, 4, t)) return rc;
+  if (t.first_block[t.n] == 0) return kOk;
+  hipLaunchKernelGGL(adamw8_pack_kernel, dim3(t.first_block[t.n]), dim3(256), 0, (hipStream_t) stream, t);
+  return check_launch(what);
+}

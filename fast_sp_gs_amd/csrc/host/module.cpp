@@ -1,6 +1,7 @@
 // Python entry points of the native host layer (fast_sp_gs_amd._host).
 #include <torch/csrc/utils/pybind.h>
 
+#include "adamw.hpp"
 #include "deform.hpp"
 #include "encode.hpp"
 #include "fast_surfel.hpp"
@@ -78,6 +79,31 @@ variable_list deform_mlp_py(const Tensor& x, const Tensor& t, const OptTensor& i
   return without_gil([&] { return deform_mlp(m, params); });
 }
 
+// element types travel by name: a torch.dtype has no C++ counterpart that pybind converts
+at::ScalarType named_type(const std::string& name) {
+  if (name == "float32") return at::kFloat;
+  if (name == "float16") return at::kHalf;
+  if (name == "bfloat16") return at::kBFloat16;
+  fail("element type " + name + " is not supported (expected float32, float16 or bfloat16)");
+}
+
+void adamw_step_py(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& m,
+                   const std::vector<Tensor>& v, const std::vector<Tensor>& steps, const std::vector<double>& lr, double b1, double b2,
+                   const std::vector<double>& eps, const std::vector<double>& decay, const OptTensor& norm) {
+  adamw_step(params, grads, m, v, steps, AdamwSettings{lr, eps, decay, b1, b2}, norm);
+}
+
+void adamw8_step_py(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& states,
+                    const std::vector<Tensor>& steps, const std::vector<double>& lr, double b1, double b2, const std::vector<double>& eps,
+                    const std::vector<double>& decay, int64_t seed, const OptTensor& norm) {
+  adamw8_step(params, grads, states, steps, AdamwSettings{lr, eps, decay, b1, b2}, seed, norm);
+}
+
+std::vector<std::pair<Tensor, Tensor>> adamw8_moments_py(const std::vector<Tensor>& states, const std::vector<Tensor>& like,
+                                                         const std::string& type) {
+  return adamw8_moments(states, like, named_type(type));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_host, m) {
@@ -95,4 +121,10 @@ PYBIND11_MODULE(_host, m) {
   m.def("image_loss", &image_loss, released);
   m.def("adam_masked_step", &adam_masked_step, released);
   m.def("adam_dense", &adam_dense, released);
+  m.def("grad_norm", &grad_norm, released);
+  m.def("adamw_step", &adamw_step_py, released);
+  m.def("adamw8_step", &adamw8_step_py, released);
+  m.def("adamw8_state_bytes", &adamw8_state_bytes);
+  m.def("adamw8_moments", &adamw8_moments_py, released);
+  m.def("adamw8_pack", &adamw8_pack, released);
 }

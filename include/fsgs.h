@@ -487,6 +487,7 @@ int fsgs_sh_to_rgb_backward_derivs(int P, int F, int degree, int clamp, const fl
 #define FSGS_DTYPE_F32 0
 #define FSGS_DTYPE_F64 1
 #define FSGS_DTYPE_F16 2
+#define FSGS_DTYPE_BF16 3 /* where an entry point names it */
 
 /* sh_encode_forward / sh_encode_backward -- fast_2d_gs/_C/src/nerf/shencoder.cu:657-691 (float, double and half, :667,
  * :688). in[B,D>=3], out[B,(C+1)^2]; the backward writes the first three components of every grad_in row. The
@@ -984,6 +985,42 @@ int fsgs_adam_masked_update_max_tensors(void);
 int fsgs_adam_masked_update_multi(int n_tensors, int64_t N, const int64_t* M, const uint8_t* mask, const double* lr,
     double b1, double b2, const double* eps, float* const* param, const float* const* grad, float* const* m,
     float* const* v, void* stream);
+
+/* ---- AdamW over many tensors (no counterpart in the reference) ------------------------------------------------------------------ */
+/* p = p (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps) after m = b1 m + (1 - b1) c g, v = b2 v + (1 - b2) (c g)^2,
+ * for up to fsgs_adamw_max_tensors() tensors of count[q] elements in one launch. Host arrays with one entry per tensor: count, step (t, the
+ * one that is being taken), lr, eps, decay and the addresses. dtype (FSGS_DTYPE_F32, _F16, _BF16) is that of param and grad; m and v are
+ * float32. norm_and_factor (device, optional): what fsgs_grad_norm_factor wrote, c = norm_and_factor[1]; 1 without it.
+ * rates (device, optional): what fsgs_adamw_rates wrote for the same tensors; step may be NULL then. Addresses need the alignment of
+ * their element type; those of four elements are moved in one access. */
+int fsgs_adamw_max_tensors(void);
+int fsgs_adamw_update_multi(int n_tensors, int dtype, const int64_t* count, const double* step, const double* lr, double b1,
+    double b2, const double* eps, const double* decay, const void* rates, const float* norm_and_factor, void* const* param,
+    const void* const* grad, float* const* m, float* const* v, void* stream);
+/* The same with both moments in 8 bits: state[q] has fsgs_adamw8_state_bytes(count[q]) bytes, 4-byte aligned, all zero before the first
+ * step. Blocks of 256 elements under one exponent per moment, the codes rounded by a hash of (element, step, seed) so that they are
+ * right on average; an infinity or a NaN among a block's moments makes all of the block's NaN. */
+size_t fsgs_adamw8_state_bytes(int64_t count);
+int fsgs_adamw8_update_multi(int n_tensors, int dtype, const int64_t* count, const double* step, const double* lr, double b1,
+    double b2, const double* eps, const double* decay, uint32_t seed, const void* rates, const float* norm_and_factor,
+    void* const* param, const void* const* grad, void* const* state, void* stream);
+/* The values that states stand for, m and v of the given dtype, and states of float32 values, rounded to nearest. */
+int fsgs_adamw8_unpack_multi(int n_tensors, int dtype, const int64_t* count, const void* const* state, void* const* m,
+    void* const* v, void* stream);
+int fsgs_adamw8_pack_multi(int n_tensors, const int64_t* count, const float* const* m, const float* const* v, void* const* state,
+    void* stream);
+/* Step counts on the device (float32, one per tensor): advances them and writes what the update needs of them to rates
+ * (fsgs_adamw_rates_bytes(n_tensors) bytes, 16-byte aligned). For steps that are captured into a graph. */
+size_t fsgs_adamw_rates_bytes(int n_tensors);
+int fsgs_adamw_rates(int n_tensors, float* const* step, const double* lr, double b1, double b2, uint32_t seed, void* rates,
+    void* stream);
+/* The norm of all gradients together: fsgs_grad_square_sums writes n_sums (at most fsgs_grad_square_sums_max()) sums of the squares of
+ * up to fsgs_adamw_max_tensors() tensors, fsgs_grad_norm_factor turns the sums of all its calls, one behind the other, into
+ * norm_and_factor[2] = {norm, min(1, max_norm / (norm + 1e-6))}. */
+int fsgs_grad_square_sums_max(void);
+int fsgs_grad_square_sums(int n_tensors, int dtype, const int64_t* count, const void* const* grad, int n_sums, double* sums,
+    void* stream);
+int fsgs_grad_norm_factor(int n_sums, const double* sums, double max_norm, float* norm_and_factor, void* stream);
 
 #ifdef __cplusplus
 }
