@@ -1,0 +1,690 @@
+// Balance of an association: how evenly points spread over the M superpoints they may belong to, with gradients.
+//
+//   P_m = (1 / T) sum_n p_nm      mean weight of a superpoint over the T points that count
+//   c_m                           how often a superpoint is chosen; f_m = c_m / sum c
+//   loss = M sum_m f_m P_m        1 where both are even, M where one superpoint takes all; f carries no gradient
+//
+// Over logits [N, M]: p_n = softmax(logits_n), chosen are a point's K largest logits, the lowest index first among equals. A row of -inf
+// alone, or one that the row mask leaves out, does not count; no entry of -inf is ever chosen. Over neighbour weights [N, K] with indices
+// [N, K]: p_n is what the weights give, chosen is the neighbour of largest weight, the first among equals.
+//
+//   d loss / d logit_nj = p_nj (a_j - sum_m p_nm a_m),   d loss / d weight_nk = a_index[n,k],   a = (g_loss M f + g_P) / T
+//
+// The pass over the rows keeps a block's sums to itself (in registers, one column's in one lane; neighbour weights as integers in LDS, where
+// the order of additions does not matter) and writes them once; a second launch adds the blocks' sums in a fixed order and forms
+// the loss: equal calls give equal results.
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+#include "../../include/fsgs.h"
+#include "common.hpp"
+
+namespace fsgs {
+namespace {
+
+constexpr int kMostChoices   = 64;
+constexpr int kPassBlocks    = 1024;  // of the pass over logits
+constexpr int kMostInLanes   = 4096;  // superpoints whose row is held by the lanes of one wavefront
+constexpr int kNeighbourBlocks = 256;
+constexpr int kNeighbourThreads = 1024;
+constexpr int kMostInLds     = 5400;  // superpoints whose sums (8 bytes) and counts (4) of a block fit in 64 KB beside a few words
+constexpr float kLog2e       = 1.44269504f;
+
+// What a block of a pass leaves: sums and counts of every superpoint, the rows that counted, whether something was no weight or no index.
+struct BlockRows {
+  int counted, invalid;
+};
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_float(__hip_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ void from_float(float x, float& y) { y = x; }
+__device__ __forceinline__ void from_float(float x, __half& y) { y = __float2half(x); }
+__device__ __forceinline__ void from_float(float x, __hip_bfloat16& y) { y = __float2bfloat16(x); }
+template <typename T, int n>
+struct alignas(n * sizeof(T)) Pack {
+  T x[n];
+};
+
+// ---- reductions over the kLanes lanes of a row; every one of them gets the result ----------------------------------------------
+template <int kCtrl>
+__device__ __forceinline__ uint32_t moved(uint32_t x) {
+  return (uint32_t) __builtin_amdgcn_update_dpp(0, (int) x, kCtrl, 0xf, 0xf, true);
+}
+__device__ __forceinline__ float as_float(uint32_t x) { return __builtin_bit_cast(float, x); }
+__device__ __forceinline__ uint32_t as_uint(float x) { return __builtin_bit_cast(uint32_t, x); }
+template <int kLanes, typename F>
+__device__ __forceinline__ uint32_t over_lanes(uint32_t x, F f) {
+  x = f(x, moved<0xB1>(x)), x = f(x, moved<0x4E>(x));                         // quad_perm: neighbours, then pairs of them
+  if (kLanes >= 16) x = f(x, moved<0x141>(x)), x = f(x, moved<0x140>(x));     // row_half_mirror, row_mirror
+  if (kLanes == 64) {
+    const uint32_t a = f(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16));
+    const uint32_t b = f(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48));
+    x = f(a, b);
+  }
+  return x;
+}
+template <int kLanes>
+__device__ __forceinline__ float row_max(float x) {
+  return as_float(over_lanes<kLanes>(as_uint(x), [](uint32_t a, uint32_t b) { return as_uint(fmaxf(as_float(a), as_float(b))); }));
+}
+template <int kLanes>
+__device__ __forceinline__ float row_sum(float x) {
+  return as_float(over_lanes<kLanes>(as_uint(x), [](uint32_t a, uint32_t b) { return as_uint(as_float(a) + as_float(b)); }));
+}
+template <int kLanes>
+__device__ __forceinline__ uint32_t row_umax(uint32_t x) {
+  return over_lanes<kLanes>(x, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+template <int kLanes>
+__device__ __forceinline__ uint32_t row_umin(uint32_t x) {
+  return over_lanes<kLanes>(x, [](uint32_t a, uint32_t b) { return min(a, b); });
+}
+template <int kLanes>
+__device__ __forceinline__ uint32_t row_count(uint32_t x) {
+  return over_lanes<kLanes>(x, [](uint32_t a, uint32_t b) { return a + b; });
+}
+
+// ---- rows of logits in the lanes of a wavefront ------------------------------------------------------------------------------------
+// kLanes lanes have a row, kVals of its columns each, in pieces of 16 bytes: piece i of lane l begins at column (i kLanes + l) 16 / size.
+template <typename T, int kLanes>
+__device__ __forceinline__ int column(int lane, int j) {
+  constexpr int kPiece = 16 / sizeof(T);
+  return (j / kPiece * kLanes + lane) * kPiece + j % kPiece;
+}
+// Columns that there are not read as -inf. `whole`: pieces are aligned, and end where the row ends.
+template <typename T, int kLanes, int kVals>
+__device__ __forceinline__ void load_row(const T* __restrict__ row, int M, bool whole, int lane, float x[kVals]) {
+  constexpr int kPiece = 16 / sizeof(T);
+#pragma unroll
+  for (int j = 0; j < kVals; j += kPiece) {
+    const int c = column<T, kLanes>(lane, j);
+    if (whole) {
+      if (c < M) {
+        const Pack<T, kPiece> q = *(const Pack<T, kPiece>*) (row + c);
+#pragma unroll
+        for (int k = 0; k < kPiece; ++k) x[j + k] = to_float(q.x[k]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < kPiece; ++k) x[j + k] = -INFINITY;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kPiece; ++k) x[j + k] = c + k < M ? to_float(row[c + k]) : -INFINITY;
+    }
+  }
+}
+
+// Counts the row's K largest values. `top`: the largest. First the K-th largest of the distinct values, K - 1 passes over registers;
+// if no more than K values reach it these are the ones. Otherwise some are equal, and they are taken one by one in order
+// of (value falling, column rising).
+template <typename T, int kLanes, int kVals>
+__device__ __forceinline__ void choose(const float x[kVals], float top, int K, int lane, int count[kVals]) {
+  float t = top;
+  for (int r = 1; r < K; ++r) {
+    float next = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kVals; ++j) next = fmaxf(next, x[j] < t ? x[j] : -INFINITY);
+    t = row_max<kLanes>(next);
+  }
+  const float least = fmaxf(t, -3.402823466e38f);  // -inf is not chosen
+  uint32_t n = 0;
+#pragma unroll
+  for (int j = 0; j < kVals; ++j) n += x[j] >= least ? 1 : 0;
+  const bool more = row_count<kLanes>(n) > (uint32_t) K;
+  if (!wave_ballot(more)) {
+#pragma unroll
+    for (int j = 0; j < kVals; ++j) count[j] += x[j] >= least ? 1 : 0;
+    return;
+  }
+  float value = INFINITY;
+  uint32_t at = 0xffffffffu;  // the last one taken: before all
+  bool first = true;
+  for (int r = 0; r < K; ++r) {
+    float best = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kVals; ++j) {
+      const bool after = first || x[j] < value || (x[j] == value && (uint32_t) column<T, kLanes>(lane, j) > at);
+      best = fmaxf(best, after ? x[j] : -INFINITY);
+    }
+    best = row_max<kLanes>(best);
+    uint32_t where = 0xffffffffu;
+#pragma unroll
+    for (int j = 0; j < kVals; ++j) {
+      const uint32_t c = (uint32_t) column<T, kLanes>(lane, j);
+      if (x[j] == best && (first || best < value || c > at)) where = min(where, c);
+    }
+    where = row_umin<kLanes>(where);
+    if (best > -INFINITY)
+#pragma unroll
+      for (int j = 0; j < kVals; ++j) count[j] += (uint32_t) column<T, kLanes>(lane, j) == where ? 1 : 0;
+    value = best, at = where, first = false;
+  }
+}
+
+template <typename T, int kLanes, int kVals>
+__global__ void __launch_bounds__(256) balance_rows_kernel(int64_t N, int M, int64_t ld, int K, const T* __restrict__ logits,
+    const uint8_t* __restrict__ rows, float2* __restrict__ stats, float* __restrict__ sums, int* __restrict__ counts,
+    BlockRows* __restrict__ blocks, unsigned* __restrict__ ticket) {
+  constexpr int kRows = 64 / kLanes;  // of a wavefront
+  __shared__ float s_sum[kLanes * kVals];
+  __shared__ int s_count[kLanes * kVals];
+  __shared__ int s_rows[4];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & (kLanes - 1), group = (threadIdx.x & 63) / kLanes;
+  const bool whole = M % (16 / sizeof(T)) == 0 && ld * sizeof(T) % 16 == 0 && ((uintptr_t) logits & 15) == 0;
+  float sum[kVals];
+  int count[kVals], counted = 0;
+#pragma unroll
+  for (int j = 0; j < kVals; ++j) sum[j] = 0.0f, count[j] = 0;
+  const int64_t step = (int64_t) gridDim.x * 4 * kRows;
+  for (int64_t base = ((int64_t) blockIdx.x * 4 + wave) * kRows; base < N; base += step) {
+    const int64_t row = base + group;
+    const bool on = row < N && (!rows || rows[row]);
+    float x[kVals];
+    if (on) {
+      load_row<T, kLanes, kVals>(logits + row * ld, M, whole, lane, x);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kVals; ++j) x[j] = -INFINITY;
+    }
+    float top = x[0];
+#pragma unroll
+    for (int j = 1; j < kVals; ++j) top = fmaxf(top, x[j]);
+    top = row_max<kLanes>(top);
+    choose<T, kLanes, kVals>(x, top, K, lane, count);
+    // a row without a number (top is -inf): the sum is 0, or NaN where one of its values is, which counts
+    const float shift = top == -INFINITY ? 0.0f : top;
+    float total = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kVals; ++j) x[j] = __builtin_amdgcn_exp2f((x[j] - shift) * kLog2e), total += x[j];
+    total = row_sum<kLanes>(total);
+    const bool counts_in = !(total == 0.0f);
+    const float scale = counts_in ? 1.0f / total : 0.0f;
+#pragma unroll
+    for (int j = 0; j < kVals; ++j) sum[j] = fmaf(x[j], scale, sum[j]);
+    if (lane == 0 && row < N) {
+      if (stats) stats[row] = make_float2(shift, scale);
+      counted += counts_in ? 1 : 0;
+    }
+  }
+  // the rows' groups of a wavefront, then the wavefronts one after the other
+#pragma unroll
+  for (int j = 0; j < kVals; ++j)
+#pragma unroll
+    for (int d = kLanes; d < 64; d <<= 1) sum[j] += __shfl_xor(sum[j], d), count[j] += __shfl_xor(count[j], d);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) counted += __shfl_xor(counted, d);
+  if ((threadIdx.x & 63) == 0) s_rows[wave] = counted;
+  for (int w = 0; w < 4; ++w) {
+    if (w == wave && group == 0)
+#pragma unroll
+      for (int j = 0; j < kVals; ++j) {
+        const int c = column<T, kLanes>(lane, j);
+        s_sum[c] = w ? s_sum[c] + sum[j] : sum[j], s_count[c] = w ? s_count[c] + count[j] : count[j];
+      }
+    __syncthreads();
+  }
+  for (int c = threadIdx.x; c < M; c += 256) {
+    sums[(size_t) blockIdx.x * M + c] = s_sum[c], counts[(size_t) blockIdx.x * M + c] = s_count[c];
+  }
+  if (threadIdx.x == 0) {
+    blocks[blockIdx.x] = BlockRows{s_rows[0] + s_rows[1] + s_rows[2] + s_rows[3], 0};
+    if (blockIdx.x == 0) *ticket = 0;
+  }
+}
+
+template <typename T, int kLanes, int kVals>
+__global__ void __launch_bounds__(256) balance_rows_backward_kernel(int64_t N, int M, int64_t ld, const T* __restrict__ logits,
+    const float2* __restrict__ stats, const int* __restrict__ counts, const int64_t* __restrict__ totals,
+    const float* __restrict__ g_loss, const float* __restrict__ g_importance, T* __restrict__ grad) {
+  constexpr int kRows = 64 / kLanes, kPiece = 16 / sizeof(T);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & (kLanes - 1), group = (threadIdx.x & 63) / kLanes;
+  const bool whole = M % kPiece == 0 && ld * sizeof(T) % 16 == 0 && ((uintptr_t) logits & 15) == 0;
+  const bool whole_out = M % kPiece == 0 && ((uintptr_t) grad & 15) == 0;
+  const float rows = (float) max(totals[1], (int64_t) 1);
+  const float of_counts = g_loss ? *g_loss * (float) M / (float) max(totals[0], (int64_t) 1) / rows : 0.0f;
+  float a[kVals];
+#pragma unroll
+  for (int j = 0; j < kVals; ++j) {
+    const int c = column<T, kLanes>(lane, j);
+    a[j] = c < M ? of_counts * (float) counts[c] + (g_importance ? g_importance[c] / rows : 0.0f) : 0.0f;
+  }
+  const int64_t step = (int64_t) gridDim.x * 4 * kRows;
+  for (int64_t base = ((int64_t) blockIdx.x * 4 + wave) * kRows; base < N; base += step) {
+    const int64_t row = base + group;
+    const float2 stat = row < N ? stats[row] : make_float2(0.0f, 0.0f);
+    const bool on = !(stat.y == 0.0f);  // a row that counted
+    float x[kVals];
+    if (on) {
+      load_row<T, kLanes, kVals>(logits + row * ld, M, whole, lane, x);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kVals; ++j) x[j] = -INFINITY;
+    }
+    float mean = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kVals; ++j) {
+      x[j] = __builtin_amdgcn_exp2f((x[j] - stat.x) * kLog2e) * stat.y;
+      mean = fmaf(x[j], a[j], mean);
+    }
+    mean = row_sum<kLanes>(mean);
+    if (row >= N) continue;
+    T* out = grad + row * M;
+#pragma unroll
+    for (int j = 0; j < kVals; j += kPiece) {
+      const int c = column<T, kLanes>(lane, j);
+      Pack<T, kPiece> q;
+#pragma unroll
+      for (int k = 0; k < kPiece; ++k) from_float(x[j + k] * (a[j + k] - mean), q.x[k]);
+      if (whole_out) {
+        if (c < M) *(Pack<T, kPiece>*) (out + c) = q;
+      } else {
+#pragma unroll
+        for (int k = 0; k < kPiece; ++k)
+          if (c + k < M) out[c + k] = q.x[k];
+      }
+    }
+  }
+}
+
+// ---- rows of more superpoints than a wavefront's lanes hold: a block a row, read again for every step -------------------------------
+template <typename F>
+__device__ __forceinline__ uint32_t over_block(uint32_t x, F f, uint32_t* s) {  // 256 threads; all get the result
+#pragma unroll
+  for (int d = 32; d; d >>= 1) x = f(x, (uint32_t) __shfl_xor((int) x, d));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = x;
+  __syncthreads();
+  return f(f(s[0], s[1]), f(s[2], s[3]));
+}
+__device__ __forceinline__ float block_max(float x, uint32_t* s) {
+  return as_float(over_block(as_uint(x), [](uint32_t a, uint32_t b) { return as_uint(fmaxf(as_float(a), as_float(b))); }, s));
+}
+__device__ __forceinline__ float block_sum(float x, uint32_t* s) {
+  return as_float(over_block(as_uint(x), [](uint32_t a, uint32_t b) { return as_uint(as_float(a) + as_float(b)); }, s));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) balance_wide_kernel(int64_t N, int M, int64_t ld, int K, const T* __restrict__ logits,
+    const uint8_t* __restrict__ rows, float2* __restrict__ stats, float* __restrict__ sums, int* __restrict__ counts,
+    BlockRows* __restrict__ blocks, unsigned* __restrict__ ticket) {
+  __shared__ uint32_t s_part[4];
+  // a column's sums belong to one thread
+  float* sum = sums + (size_t) blockIdx.x * M;
+  int *count = counts + (size_t) blockIdx.x * M, counted = 0;
+  for (int c = threadIdx.x; c < M; c += 256) sum[c] = 0.0f, count[c] = 0;
+  for (int64_t row = blockIdx.x; row < N; row += gridDim.x) {
+    const T* x = logits + row * ld;
+    const bool on = !rows || rows[row];
+    float top = -INFINITY, total = 0.0f;
+    if (on) {
+      for (int c = threadIdx.x; c < M; c += 256) top = fmaxf(top, to_float(x[c]));
+      top = block_max(top, s_part);
+    }
+    const float shift = top == -INFINITY ? 0.0f : top;
+    if (on) {
+      for (int c = threadIdx.x; c < M; c += 256) total += __builtin_amdgcn_exp2f((to_float(x[c]) - shift) * kLog2e);
+      total = block_sum(total, s_part);
+    }
+    const bool counts_in = !(total == 0.0f);
+    const float scale = counts_in ? 1.0f / total : 0.0f;
+    if (threadIdx.x == 0 && stats) stats[row] = make_float2(shift, scale);
+    if (!counts_in) continue;
+    ++counted;
+    for (int c = threadIdx.x; c < M; c += 256) sum[c] += __builtin_amdgcn_exp2f((to_float(x[c]) - shift) * kLog2e) * scale;
+    float value = INFINITY;
+    uint32_t at = 0;
+    for (int r = 0; r < K; ++r) {
+      float best = -INFINITY;
+      uint32_t where = 0xffffffffu;
+      for (int c = threadIdx.x; c < M; c += 256) {
+        const float y = to_float(x[c]);
+        const bool after = r == 0 || y < value || (y == value && (uint32_t) c > at);
+        if (after && y > best) best = y, where = (uint32_t) c;
+      }
+      const float most = block_max(best, s_part);
+      if (!(most > -INFINITY)) break;
+      where = over_block(best == most ? where : 0xffffffffu, [](uint32_t a, uint32_t b) { return min(a, b); }, s_part);
+      if (where % 256 == threadIdx.x) ++count[where];
+      value = most, at = where;
+    }
+  }
+  if (threadIdx.x == 0) {
+    blocks[blockIdx.x] = BlockRows{counted, 0};
+    if (blockIdx.x == 0) *ticket = 0;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) balance_wide_backward_kernel(int64_t N, int M, int64_t ld, const T* __restrict__ logits,
+    const float2* __restrict__ stats, const int* __restrict__ counts, const int64_t* __restrict__ totals,
+    const float* __restrict__ g_loss, const float* __restrict__ g_importance, T* __restrict__ grad) {
+  __shared__ uint32_t s_part[4];
+  const float rows = (float) max(totals[1], (int64_t) 1);
+  const float of_counts = g_loss ? *g_loss * (float) M / (float) max(totals[0], (int64_t) 1) / rows : 0.0f;
+  auto slope = [&](int c) { return of_counts * (float) counts[c] + (g_importance ? g_importance[c] / rows : 0.0f); };
+  for (int64_t row = blockIdx.x; row < N; row += gridDim.x) {
+    const float2 stat = stats[row];
+    const T* x = logits + row * ld;
+    T* out = grad + row * M;
+    const bool on = !(stat.y == 0.0f);
+    auto weight = [&](int c) { return __builtin_amdgcn_exp2f((to_float(x[c]) - stat.x) * kLog2e) * stat.y; };
+    float mean = 0.0f;
+    if (on) {
+      for (int c = threadIdx.x; c < M; c += 256) mean = fmaf(weight(c), slope(c), mean);
+      mean = block_sum(mean, s_part);
+    }
+    for (int c = threadIdx.x; c < M; c += 256) from_float(on ? weight(c) * (slope(c) - mean) : 0.0f, out[c]);
+  }
+}
+
+// ---- neighbour weights ----------------------------------------------------------------------------------------------------------------
+// Weights lie in [0, 1] (a rounding above 1 is let pass): in units of 2^-31 a block's sums are integers of 64 bits. A weight that is none,
+// or an index that is none, is reported and left out.
+constexpr float kWeightUnits = 2147483648.0f;
+
+template <bool kLds>
+__global__ void __launch_bounds__(kNeighbourThreads) balance_neighbours_kernel(int64_t N, int M, int K,
+    const float* __restrict__ weights, const int64_t* __restrict__ indices, const uint8_t* __restrict__ rows,
+    unsigned long long* __restrict__ sums, int* __restrict__ counts, BlockRows* __restrict__ blocks, unsigned* __restrict__ ticket) {
+  extern __shared__ unsigned long long s_sums[];  // [M], then the counts [M]
+  __shared__ int s_rows[2];
+  unsigned long long* sum = kLds ? s_sums : sums;
+  int* count = kLds ? (int*) (s_sums + M) : counts;
+  if (kLds)
+    for (int c = threadIdx.x; c < M; c += kNeighbourThreads) sum[c] = 0, count[c] = 0;
+  if (threadIdx.x < 2) s_rows[threadIdx.x] = 0;
+  __syncthreads();
+  int counted = 0, invalid = 0;
+  for (int64_t n = (int64_t) blockIdx.x * kNeighbourThreads + threadIdx.x; n < N; n += (int64_t) gridDim.x * kNeighbourThreads) {
+    if (rows && !rows[n]) continue;
+    ++counted;
+    float best = -1.0f;
+    int64_t where = 0;
+    for (int k = 0; k < K; ++k) {
+      const float w = weights[n * K + k];
+      const int64_t m = indices[n * K + k];
+      if (!(w >= 0.0f && w <= 1.0001f) || m < 0 || m >= M) {
+        invalid = 1;
+        continue;
+      }
+      atomicAdd(&sum[m], (unsigned long long) (uint32_t) __float2uint_rn(w * kWeightUnits));
+      if (w > best) best = w, where = m;
+    }
+    if (best >= 0.0f) atomicAdd(&count[where], 1);
+  }
+  if (counted) atomicAdd(&s_rows[0], counted);
+  if (invalid) atomicOr(&s_rows[1], 1);
+  __syncthreads();
+  if (kLds)
+    for (int c = threadIdx.x; c < M; c += kNeighbourThreads)
+      sums[(size_t) blockIdx.x * M + c] = sum[c], counts[(size_t) blockIdx.x * M + c] = count[c];
+  if (threadIdx.x == 0) {
+    blocks[blockIdx.x] = BlockRows{s_rows[0], s_rows[1]};
+    if (blockIdx.x == 0) *ticket = 0;
+  }
+}
+
+__global__ void __launch_bounds__(256) balance_neighbours_backward_kernel(int64_t N, int M, int K, const int64_t* __restrict__ indices,
+    const uint8_t* __restrict__ rows, const int* __restrict__ counts, const int64_t* __restrict__ totals,
+    const float* __restrict__ g_loss, const float* __restrict__ g_importance, float* __restrict__ grad) {
+  const float of_rows = (float) max(totals[1], (int64_t) 1);
+  const float of_counts = g_loss ? *g_loss * (float) M / (float) max(totals[0], (int64_t) 1) / of_rows : 0.0f;
+  for (int64_t e = (int64_t) blockIdx.x * 256 + threadIdx.x; e < N * K; e += (int64_t) gridDim.x * 256) {
+    float g = 0.0f;
+    if (!rows || rows[e / K]) {
+      const int64_t m = indices[e];
+      if (m < 0 || m >= M) g = __builtin_nanf("");
+      else g = of_counts * (float) counts[m] + (g_importance ? g_importance[m] / of_rows : 0.0f);
+    }
+    grad[e] = g;
+  }
+}
+
+__global__ void __launch_bounds__(256) clear_kernel(int M, unsigned long long* sums, int* counts) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c < M) sums[c] = 0, counts[c] = 0;
+}
+
+// ---- the blocks' sums together -----------------------------------------------------------------------------------------------------------
+// A block takes 32 superpoints, 32 threads of it a superpoint's blocks in turn; the last block to end forms the loss of all of them.
+__device__ __forceinline__ double value_of(float s) { return (double) s; }
+__device__ __forceinline__ double value_of(unsigned long long s) { return (double) s * (1.0 / kWeightUnits); }
+__device__ __forceinline__ double added(double a, float s) { return a + (double) s; }
+__device__ __forceinline__ unsigned long long added(unsigned long long a, unsigned long long s) { return a + s; }
+template <typename S> struct TotalOf { using type = double; };
+template <> struct TotalOf<unsigned long long> { using type = unsigned long long; };
+__device__ __forceinline__ double value_of(double s) { return s; }
+
+template <typename S>
+__global__ void __launch_bounds__(1024) balance_totals_kernel(int G, int G_rows, int M, const S* __restrict__ sums,
+    const int* __restrict__ block_counts, const BlockRows* __restrict__ blocks, double* __restrict__ parts, unsigned* __restrict__ ticket,
+    float* __restrict__ loss, int* __restrict__ counts, float* __restrict__ importance, int64_t* __restrict__ totals) {
+  using Total = typename TotalOf<S>::type;
+  __shared__ Total s_sum[32][33];
+  __shared__ int s_count[32][33];
+  __shared__ int s_rows, s_invalid, s_last;
+  const int c = threadIdx.x & 31, slice = threadIdx.x >> 5, m = blockIdx.x * 32 + c;
+  if (threadIdx.x == 0) s_rows = 0, s_invalid = 0;
+  Total sum = 0;
+  int count = 0;
+  if (m < M)
+#pragma unroll 8
+    for (int g = slice; g < G; g += 32) sum = added(sum, sums[(size_t) g * M + m]), count += block_counts[(size_t) g * M + m];
+  s_sum[slice][c] = sum, s_count[slice][c] = count;
+  __syncthreads();
+  for (int g = threadIdx.x; g < G_rows; g += 1024) {
+    atomicAdd(&s_rows, blocks[g].counted);
+    if (blocks[g].invalid) s_invalid = 1;
+  }
+  __syncthreads();
+  const int T = s_rows, of = max(T, 1);
+  if (threadIdx.x < 64) {  // a wavefront: the slices in order, then the block's share of the loss
+    double chosen = 0.0, both = 0.0;
+    if (slice == 0 && m < M) {
+      for (int k = 1; k < 32; ++k) sum += s_sum[k][c], count += s_count[k][c];
+      const double s = s_invalid ? __builtin_nan("") : value_of(sum);
+      counts[m] = count, importance[m] = (float) (s / of);
+      chosen = (double) count, both = (double) count * s;
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) chosen += __shfl_xor(chosen, d), both += __shfl_xor(both, d);
+    if (threadIdx.x == 0) {
+      parts[2 * blockIdx.x] = chosen, parts[2 * blockIdx.x + 1] = both;
+      __threadfence();
+      s_last = atomicAdd(ticket, 1u) == gridDim.x - 1;
+    }
+  }
+  __syncthreads();
+  if (!s_last || threadIdx.x >= 64) return;
+  __threadfence();
+  double chosen = 0.0, both = 0.0;
+  for (int b = threadIdx.x; b < (int) gridDim.x; b += 64)
+    chosen += __builtin_nontemporal_load(parts + 2 * b), both += __builtin_nontemporal_load(parts + 2 * b + 1);
+#pragma unroll
+  for (int d = 32; d; d >>= 1) chosen += __shfl_xor(chosen, d), both += __shfl_xor(both, d);
+  if (threadIdx.x == 0) {
+    *loss = (float) ((double) M * both / ((chosen > 0.0 ? chosen : 1.0) * (double) of));
+    totals[0] = (int64_t) chosen, totals[1] = T;
+  }
+}
+
+// ---- launches -------------------------------------------------------------------------------------------------------------------------------
+struct Workspace {
+  size_t counts, blocks, parts, ticket, bytes;  // sums come first
+  Workspace(int G, int64_t M, size_t sum_bytes, int G_rows) {
+    counts = align_up((size_t) G * M * sum_bytes, 256);
+    blocks = counts + align_up((size_t) G * M * 4, 256);
+    parts  = blocks + align_up((size_t) G_rows * sizeof(BlockRows), 256);
+    ticket = parts + align_up((size_t) div_up(M, 32) * 16, 256);
+    bytes  = ticket + 256;
+  }
+};
+
+// Lanes a row, by its bytes: the fewest of 4, 16 and 64 that hold it in 32 values each (16 values for 4 lanes).
+int lanes_of(int M, int piece) { return M <= 4 * piece ? 4 : M <= 512 ? 16 : 64; }
+int pass_blocks(int64_t N, int M, int dtype) {
+  if (N == 0) return 0;
+  const int rows = M > kMostInLanes ? 1 : 4 * (64 / lanes_of(M, dtype == FSGS_DTYPE_F32 ? 4 : 8));
+  const int64_t blocks = (N + rows - 1) / rows;
+  return (int) (blocks < kPassBlocks ? blocks : kPassBlocks);
+}
+bool in_lds(int64_t M) { return M <= kMostInLds; }
+int neighbour_blocks(int64_t N) {
+  const int64_t blocks = (N + kNeighbourThreads - 1) / kNeighbourThreads;
+  return (int) (blocks < kNeighbourBlocks ? blocks : kNeighbourBlocks);
+}
+
+// kernel<T, lanes, values>(...) for the narrowest rows that hold M columns
+#define FSGS_ROW_KERNELS(T, LAUNCH)                      \
+  do {                                                   \
+    constexpr int kPiece = 16 / sizeof(T);               \
+    if (M <= 4 * kPiece) LAUNCH(T, 4, kPiece);           \
+    else if (kPiece == 4 && M <= 64) LAUNCH(T, 16, 4 * (kPiece / 4)); \
+    else if (M <= 128) LAUNCH(T, 16, 8);                 \
+    else if (M <= 256) LAUNCH(T, 16, 16);                \
+    else if (M <= 512) LAUNCH(T, 16, 32);                \
+    else if (M <= 1024) LAUNCH(T, 64, 16);               \
+    else if (M <= 2048) LAUNCH(T, 64, 32);               \
+    else LAUNCH(T, 64, 64);                              \
+  } while (0)
+
+template <typename T>
+void launch_rows(int G, int64_t N, int M, int64_t ld, int K, const void* logits, const uint8_t* rows, float2* stats, float* sums,
+                 int* counts, BlockRows* blocks, unsigned* ticket, hipStream_t s) {
+  const T* x = (const T*) logits;
+#define LAUNCH(T, L, V) \
+  hipLaunchKernelGGL((balance_rows_kernel<T, L, V>), dim3(G), dim3(256), 0, s, N, M, ld, K, x, rows, stats, sums, counts, blocks, ticket)
+  if (M > kMostInLanes)
+    hipLaunchKernelGGL((balance_wide_kernel<T>), dim3(G), dim3(256), 0, s, N, M, ld, K, x, rows, stats, sums, counts, blocks, ticket);
+  else
+    FSGS_ROW_KERNELS(T, LAUNCH);
+#undef LAUNCH
+}
+
+template <typename T>
+void launch_rows_backward(int G, int64_t N, int M, int64_t ld, const void* logits, const float2* stats, const int* counts,
+                          const int64_t* totals, const float* g_loss, const float* g_importance, void* grad, hipStream_t s) {
+  const T* x = (const T*) logits;
+  T* out = (T*) grad;
+#define LAUNCH(T, L, V)                                                                                                            \
+  hipLaunchKernelGGL((balance_rows_backward_kernel<T, L, V>), dim3(G), dim3(256), 0, s, N, M, ld, x, stats, counts, totals, g_loss, \
+                     g_importance, out)
+  if (M > kMostInLanes)
+    hipLaunchKernelGGL((balance_wide_backward_kernel<T>), dim3(G), dim3(256), 0, s, N, M, ld, x, stats, counts, totals, g_loss,
+                       g_importance, out);
+  else
+    FSGS_ROW_KERNELS(T, LAUNCH);
+#undef LAUNCH
+}
+#undef FSGS_ROW_KERNELS
+
+bool is_type(int type) { return type == FSGS_DTYPE_F32 || type == FSGS_DTYPE_F16 || type == FSGS_DTYPE_BF16; }
+
+}  // namespace
+}  // namespace fsgs
+
+using namespace fsgs;
+
+FSGS_API int fsgs_balance_max_choices(void) { return kMostChoices; }
+
+FSGS_API size_t fsgs_balance_loss_workspace_bytes(int64_t N, int M, int dtype) {
+  if (N < 0 || M <= 0) return 0;
+  const int G = pass_blocks(N, M, dtype);
+  return Workspace(G, M, 4, G).bytes;
+}
+
+FSGS_API int fsgs_balance_loss_forward(int64_t N, int M, int64_t ld, int K, int dtype, const void* logits, const uint8_t* rows,
+    float* loss, int32_t* counts, float* importance, int64_t* totals, float* stats, void* workspace, size_t workspace_bytes,
+    void* stream) {
+  const char* what = "balance_loss";
+  FSGS_REQUIRE(N >= 0 && N < (int64_t) 0x7fffffff && M > 0 && is_type(dtype) && (N <= 1 || ld >= M), "%s: bad arguments", what);
+  FSGS_REQUIRE(K >= 1 && K <= M && K <= kMostChoices, "%s: K must be in [1, min(M, %d)]", what, kMostChoices);
+  FSGS_REQUIRE((N == 0 || logits) && loss && counts && importance && totals && workspace, "%s: null pointer", what);
+  FSGS_REQUIRE((uintptr_t) logits % (dtype == FSGS_DTYPE_F32 ? 4 : 2) == 0 && (uintptr_t) stats % 8 == 0 && (uintptr_t) workspace % 8 == 0,
+               "%s: misaligned address", what);
+  const int G = pass_blocks(N, M, dtype);
+  const Workspace ws(G, M, 4, G);
+  if (workspace_bytes < ws.bytes) return fsgs::fail(kWorkspaceSmall, "%s: the workspace is too small", what);
+  char* at = (char*) workspace;
+  float* sums = (float*) at;
+  int* block_counts = (int*) (at + ws.counts);
+  BlockRows* blocks = (BlockRows*) (at + ws.blocks);
+  unsigned* ticket = (unsigned*) (at + ws.ticket);
+  hipStream_t s = (hipStream_t) stream;
+  if (G == 0) {
+    hipLaunchKernelGGL(clear_kernel, dim3(1), dim3(256), 0, s, 1, (unsigned long long*) ticket, (int*) ticket + 2);
+  } else {
+    auto launch = dtype == FSGS_DTYPE_F32 ? launch_rows<float> : dtype == FSGS_DTYPE_F16 ? launch_rows<__half> : launch_rows<__hip_bfloat16>;
+    launch(G, N, M, ld, K, logits, rows, (float2*) stats, sums, block_counts, blocks, ticket, s);
+  }
+  if (const int rc = check_launch(what)) return rc;
+  hipLaunchKernelGGL(balance_totals_kernel<float>, dim3(div_up(M, 32)), dim3(1024), 0, s, G, G, M, sums, block_counts, blocks,
+                     (double*) (at + ws.parts), ticket, loss, counts, importance, totals);
+  return check_launch(what);
+}
+
+FSGS_API int fsgs_balance_loss_backward(int64_t N, int M, int64_t ld, int dtype, const void* logits, const float* stats,
+    const int32_t* counts, const int64_t* totals, const float* g_loss, const float* g_importance, void* grad, void* stream) {
+  const char* what = "balance_loss_backward";
+  FSGS_REQUIRE(N >= 0 && N < (int64_t) 0x7fffffff && M > 0 && is_type(dtype) && (N <= 1 || ld >= M), "%s: bad arguments", what);
+  if (N == 0) return kOk;
+  FSGS_REQUIRE(logits && stats && counts && totals && grad && (g_loss || g_importance), "%s: null pointer", what);
+  const size_t size = dtype == FSGS_DTYPE_F32 ? 4 : 2;
+  FSGS_REQUIRE(((uintptr_t) logits | (uintptr_t) grad) % size == 0 && (uintptr_t) stats % 8 == 0, "%s: misaligned address", what);
+  const int rows = M > kMostInLanes ? 1 : 4 * (64 / lanes_of(M, (int) (16 / size)));
+  const int64_t blocks = (N + rows - 1) / rows;
+  const int G = (int) (blocks < 4096 ? blocks : 4096);
+  auto launch = dtype == FSGS_DTYPE_F32 ? launch_rows_backward<float> : dtype == FSGS_DTYPE_F16 ? launch_rows_backward<__half> : launch_rows_backward<__hip_bfloat16>;
+  launch(G, N, M, ld, logits, (const float2*) stats, counts, totals, g_loss, g_importance, grad, (hipStream_t) stream);
+  return check_launch(what);
+}
+
+FSGS_API size_t fsgs_neighbour_balance_workspace_bytes(int64_t N, int M) {
+  if (N < 0 || M <= 0) return 0;
+  const int G = neighbour_blocks(N);
+  return Workspace(in_lds(M) ? G : 1, M, 8, G).bytes;
+}
+
+FSGS_API int fsgs_neighbour_balance_forward(int64_t N, int M, int K, const float* weights, const int64_t* indices, const uint8_t* rows,
+    float* loss, int32_t* counts, float* importance, int64_t* totals, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "neighbour_balance";
+  FSGS_REQUIRE(N >= 0 && N < (int64_t) 0x7fffffff && M > 0 && K >= 1, "%s: bad arguments", what);
+  FSGS_REQUIRE((N == 0 || (weights && indices)) && loss && counts && importance && totals && workspace, "%s: null pointer", what);
+  FSGS_REQUIRE((uintptr_t) weights % 4 == 0 && (uintptr_t) indices % 8 == 0 && (uintptr_t) workspace % 8 == 0, "%s: misaligned address", what);
+  const int G = neighbour_blocks(N), G_sums = in_lds(M) ? G : 1;
+  const Workspace ws(G_sums, M, 8, G);
+  if (workspace_bytes < ws.bytes) return fsgs::fail(kWorkspaceSmall, "%s: the workspace is too small", what);
+  char* at = (char*) workspace;
+  unsigned long long* sums = (unsigned long long*) at;
+  int* block_counts = (int*) (at + ws.counts);
+  BlockRows* blocks = (BlockRows*) (at + ws.blocks);
+  unsigned* ticket = (unsigned*) (at + ws.ticket);
+  hipStream_t s = (hipStream_t) stream;
+  if (!in_lds(M)) hipLaunchKernelGGL(clear_kernel, dim3(div_up(M, 256)), dim3(256), 0, s, M, sums, block_counts);
+  if (G == 0)
+    hipLaunchKernelGGL(clear_kernel, dim3(1), dim3(256), 0, s, 1, (unsigned long long*) ticket, (int*) ticket + 2);
+  else if (in_lds(M))
+    hipLaunchKernelGGL(balance_neighbours_kernel<true>, dim3(G), dim3(kNeighbourThreads), (size_t) M * 12, s, N, M, K, weights, indices,
+                       rows, sums, block_counts, blocks, ticket);
+  else
+    hipLaunchKernelGGL(balance_neighbours_kernel<false>, dim3(G), dim3(kNeighbourThreads), 0, s, N, M, K, weights, indices, rows, sums,
+                       block_counts, blocks, ticket);
+  if (const int rc = check_launch(what)) return rc;
+  hipLaunchKernelGGL(balance_totals_kernel<unsigned long long>, dim3(div_up(M, 32)), dim3(1024), 0, s, G_sums, G, M, sums, block_counts,
+                     blocks, (double*) (at + ws.parts), ticket, loss, counts, importance, totals);
+  return check_launch(what);
+}
+
+FSGS_API int fsgs_neighbour_balance_backward(int64_t N, int M, int K, const int64_t* indices, const uint8_t* rows,
+    const int32_t* counts, const int64_t* totals, const float* g_loss, const float* g_importance, float* grad, void* stream) {
+  const char* what = "neighbour_balance_backward";
+  FSGS_REQUIRE(N >= 0 && N < (int64_t) 0x7fffffff && M > 0 && K >= 1, "%s: bad arguments", what);
+  if (N == 0) return kOk;
+  FSGS_REQUIRE(indices && counts && totals && grad && (g_loss || g_importance), "%s: null pointer", what);
+  FSGS_REQUIRE((uintptr_t) indices % 8 == 0 && (uintptr_t) grad % 4 == 0, "%s: misaligned address", what);
+  const int64_t blocks = (N * K + 255) / 256;
+  hipLaunchKernelGGL(balance_neighbours_backward_kernel, dim3((unsigned) (blocks < 8192 ? blocks : 8192)), dim3(256), 0,
+                     (hipStream_t) stream, N, M, K, indices, rows, counts, totals, g_loss, g_importance, grad);
+  return check_launch(what);
+}

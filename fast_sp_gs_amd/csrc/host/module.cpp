@@ -2,6 +2,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include "adamw.hpp"
+#include "balance.hpp"
 #include "deform.hpp"
 #include "encode.hpp"
 #include "fast_surfel.hpp"
@@ -127,4 +128,6 @@ PYBIND11_MODULE(_host, m) {
   m.def("adamw8_state_bytes", &adamw8_state_bytes);
   m.def("adamw8_moments", &adamw8_moments_py, released);
   m.def("adamw8_pack", &adamw8_pack, released);
+  m.def("balance_loss", &balance_loss, released);
+  m.def("neighbour_balance", &neighbour_balance, released);
 }

@@ -1022,6 +1022,28 @@ int fsgs_grad_square_sums(int n_tensors, int dtype, const int64_t* count, const 
     void* stream);
 int fsgs_grad_norm_factor(int n_sums, const double* sums, double max_norm, float* norm_and_factor, void* stream);
 
+/* ---- balance of an association (no counterpart in the reference) ------------------------------------------------------------------ */
+/* loss[] = M sum_m f_m P_m, counts[M], importance[M] = P and totals[2] = {choices, rows that count} of logits [N, M] (dtype as above, rows
+ * ld elements apart): P the mean softmax over the rows that count, f a superpoint's share of the choices, each row choosing its K largest
+ * logits above -inf, the lowest index first (K <= fsgs_balance_max_choices()). rows[N] (optional): 0 leaves a row out, unread. stats[N][2]
+ * (optional, 8-byte aligned): what the backward needs of each row. workspace: fsgs_balance_loss_workspace_bytes bytes, 8-byte aligned.
+ * The backward writes grad[N, M] (dtype, contiguous) = p (a - sum p a), a = (g_loss M f + g_importance) / T; either of the two upstream
+ * gradients (device, g_loss one float, g_importance[M]) may be NULL. N < 2^31. */
+int fsgs_balance_max_choices(void);
+size_t fsgs_balance_loss_workspace_bytes(int64_t N, int M, int dtype);
+int fsgs_balance_loss_forward(int64_t N, int M, int64_t ld, int K, int dtype, const void* logits, const uint8_t* rows,
+    float* loss, int32_t* counts, float* importance, int64_t* totals, float* stats, void* workspace, size_t workspace_bytes,
+    void* stream);
+int fsgs_balance_loss_backward(int64_t N, int M, int64_t ld, int dtype, const void* logits, const float* stats,
+    const int32_t* counts, const int64_t* totals, const float* g_loss, const float* g_importance, void* grad, void* stream);
+/* The same of weights[N, K] in [0, 1] with indices[N, K] in [0, M): a row chooses its largest weight, the first of equal ones. A weight or
+ * an index outside, in a row that counts, makes loss and importance NaN. The backward's grad[N, K] = a[index], 0 in rows left out. */
+size_t fsgs_neighbour_balance_workspace_bytes(int64_t N, int M);
+int fsgs_neighbour_balance_forward(int64_t N, int M, int K, const float* weights, const int64_t* indices, const uint8_t* rows,
+    float* loss, int32_t* counts, float* importance, int64_t* totals, void* workspace, size_t workspace_bytes, void* stream);
+int fsgs_neighbour_balance_backward(int64_t N, int M, int K, const int64_t* indices, const uint8_t* rows,
+    const int32_t* counts, const int64_t* totals, const float* g_loss, const float* g_importance, float* grad, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
