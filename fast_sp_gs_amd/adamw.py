@@ -77,7 +77,8 @@ def adamw8_state(param: Tensor) -> Tensor:
 
 def adamw8_moments(states: Sequence[Tensor], like: Sequence[Tensor], dtype: torch.dtype = torch.float32) -> List[Tuple[Tensor, Tensor]]:
     """(m, v) that the states stand for, in the shapes of the tensors `like` that they belong to. The values have at most four
-    significant bits: they are exact in any of the types unless a block's scale takes them out of float16's range."""
+    significant bits: they are exact in any of the types unless a block's scale takes them out of float16's range. They are parts of one
+    allocation."""
     return host.adamw8_moments(list(states), list(like), str(dtype).replace('torch.', ''))
 
 

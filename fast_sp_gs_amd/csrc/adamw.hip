@@ -113,12 +113,14 @@ struct Step {
   float b1, b2, c1, c2;  // c = 1 - b
 };
 
-// One element; the moments are replaced. Every operation rounds by itself, as a chain of tensor operations does.
+// One element; the moments are replaced. The root and the reciprocal are the hardware's, one unit in the last place each. The root's
+// instruction takes subnormal numbers for 0, so v counts as 2^-126 at least: the smallest root is 1e-19, a hundred-thousandth of an eps
+// of 1e-15 (scenes' own), and nothing is divided by 0 where eps is. A NaN stays one.
 __device__ __forceinline__ float updated(const Step& s, const Rates& r, float keep, float eps, float p, float g, float& m, float& v) {
-#pragma clang fp contract(off)
-  m = s.b1 * m + s.c1 * g;
-  v = s.b2 * v + s.c2 * g * g;
-  return p * keep - r.step_size * m / (sqrtf(v) * r.inv_root_c2 + eps);
+  m = fmaf(s.c1, g, s.b1 * m);
+  v = fmaf(s.c2 * g, g, s.b2 * v);
+  const float root = __builtin_amdgcn_sqrtf(v < 0x1p-126f ? 0x1p-126f : v);
+  return fmaf(p, keep, -(r.step_size * m * __builtin_amdgcn_rcpf(fmaf(root, r.inv_root_c2, eps))));
 }
 
 // ---- 32-bit moments -------------------------------------------------------------------------------------------------------------
@@ -167,14 +169,32 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
 
 // From a code's place in a float32 (exponent 1 is its lowest binade) to that of its block, whose highest one is 2^kBits - 1.
 template <int kBits>  // of exponent
-__device__ __forceinline__ float decoded(uint32_t code, int exponent) {
-  const float x = ldexpf(__builtin_bit_cast(float, code << 20), exponent + 1 - (1 << kBits));
-  return exponent == 255 ? __builtin_nanf("") : x;
+__device__ __forceinline__ float decoded(uint32_t bits, int exponent) {
+  return ldexpf(__builtin_bit_cast(float, bits), exponent + 1 - (1 << kBits));
 }
 template <int kBits>
-__device__ __forceinline__ uint32_t encoded(float x, int exponent, uint32_t noise16) {
+__device__ __forceinline__ uint32_t encoded(float x, int exponent, uint32_t noise16, uint32_t least) {
   const uint32_t y = __builtin_bit_cast(uint32_t, ldexpf(x, (1 << kBits) - 1 - exponent));
-  return min((y + (noise16 << 4)) >> 20, (8u << kBits) - 1);
+  return min(max((y + (noise16 << 4)) >> 20, least), (8u << kBits) - 1);
+}
+// Element k of the four whose codes are in a word each.
+template <int k>
+__device__ __forceinline__ void decode(uint32_t codes_m, uint32_t codes_v, int exponent_m, int exponent_v, float& m, float& v) {
+  // a code's magnitude to bits 20 to 26 (m) or 27 (v), m's sign to bit 31
+  const uint32_t a = k == 0 ? codes_m << 20 : k == 1 ? codes_m << 12 : k == 2 ? codes_m << 4 : codes_m >> 4;
+  const uint32_t b = k == 0 ? codes_v << 20 : k == 1 ? codes_v << 12 : k == 2 ? codes_v << 4 : codes_v >> 4;
+  m = decoded<4>((a & 0x07f00000u) | ((codes_m << (24 - 8 * k)) & 0x80000000u), exponent_m);
+  v = decoded<5>(b & 0x0ff00000u, exponent_v);
+}
+__device__ __forceinline__ void decode4(uint32_t codes_m, uint32_t codes_v, int exponent_m, int exponent_v, float m[4], float v[4]) {
+  decode<0>(codes_m, codes_v, exponent_m, exponent_v, m[0], v[0]), decode<1>(codes_m, codes_v, exponent_m, exponent_v, m[1], v[1]);
+  decode<2>(codes_m, codes_v, exponent_m, exponent_v, m[2], v[2]), decode<3>(codes_m, codes_v, exponent_m, exponent_v, m[3], v[3]);
+  if (exponent_m == 255)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m[k] = __builtin_nanf("");
+  if (exponent_v == 255)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = __builtin_nanf("");
 }
 // A block's exponent byte from the bits of its largest magnitude (a NaN is larger than any): that of the next binade where the value is
 // above 1.875 of its own. Below the normal numbers the lowest normal exponent stands for all; 254 is the last of finite values.
@@ -196,10 +216,10 @@ __device__ __forceinline__ void encode4(const float m[4], const float v[4], cons
   codes_m = codes_v = 0;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const uint32_t a = encoded<4>(fabsf(m[k]), exponent_m, noise[k] & 0xffffu);
-    uint32_t b = encoded<5>(v[k], exponent_v, noise[k] >> 16);
-    if (b == 0 && v[k] > 0.0f) b = 1;
-    codes_m |= (a | (m[k] < 0.0f && a ? 128u : 0u)) << (8 * k);
+    const uint32_t bits_m = __builtin_bit_cast(uint32_t, m[k]), bits_v = __builtin_bit_cast(uint32_t, v[k]);
+    const uint32_t a = encoded<4>(fabsf(m[k]), exponent_m, noise[k] & 0xffffu, 0);
+    const uint32_t b = encoded<5>(v[k], exponent_v, noise[k] >> 16, min(bits_v, 1u));
+    codes_m |= (a | ((bits_m >> 24) & 128u)) << (8 * k);
     codes_v |= b << (8 * k);
   }
 }
@@ -213,17 +233,12 @@ __host__ __device__ __forceinline__ StateView view_state(void* state, int64_t co
   return {at, at + b * kBlock, at + 2 * b * kBlock};
 }
 
-__device__ __forceinline__ void decode(uint32_t a, uint32_t b, int exponent_m, int exponent_v, float& m, float& v) {
-  m = decoded<4>(a & 127, exponent_m), v = decoded<5>(b & 255, exponent_v);
-  if (a & 128) m = -m;
-}
-
 // A wavefront steps a block: a lane has four elements of it.
 template <typename T>
 __global__ void __launch_bounds__(256) adamw8_kernel(AdamwTable t, Step s, const float* __restrict__ factor,
                                                      const Rates* __restrict__ rates) {
   const int q = tensor_of(t.first_block, t.n, blockIdx.x);
-  const int64_t block = (int64_t) (blockIdx.x - t.first_block[q]) * 4 + (threadIdx.x >> 6);
+  const int64_t block = (int64_t) (blockIdx.x - t.first_block[q]) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   if (block * kBlock >= t.count[q]) return;  // the whole wavefront
   const int64_t e = block * kBlock + lane * 4, left = t.count[q] - e;
@@ -237,10 +252,10 @@ __global__ void __launch_bounds__(256) adamw8_kernel(AdamwTable t, Step s, const
   load4(param, left, whole, p), load4(grad, left, whole, g);
   const uint32_t old_m = *(const uint32_t*) (state.m + e), old_v = *(const uint32_t*) (state.v + e);
   int exponent_m = state.exponents[2 * block], exponent_v = state.exponents[2 * block + 1];
+  decode4(old_m, old_v, exponent_m, exponent_v, m, v);
   uint32_t noise[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    decode(old_m >> (8 * k), old_v >> (8 * k), exponent_m, exponent_v, m[k], v[k]);
     p[k] = updated(s, rate, keep, eps, p[k], c * g[k], m[k], v[k]);
     if (k >= left) m[k] = v[k] = 0.0f;
     noise[k] = mixed((uint32_t) (e + k) * kStride + rate.key);
@@ -261,21 +276,32 @@ struct MomentsTable {
   int n;
 };
 
-// The values that 8-bit moments stand for.
+// The values that 8-bit moments stand for; a lane writes 16 bytes of each.
 template <typename T>
 __global__ void __launch_bounds__(256) adamw8_unpack_kernel(MomentsTable t) {
+  constexpr int kWords = 4 / sizeof(T);  // of four codes
   const int q = tensor_of(t.first_block, t.n, blockIdx.x);
-  const int64_t e = (int64_t) (blockIdx.x - t.first_block[q]) * 1024 + threadIdx.x * 4, left = t.count[q] - e;
+  const int64_t e = ((int64_t) (blockIdx.x - t.first_block[q]) * 256 + threadIdx.x) * 4 * kWords, left = t.count[q] - e;
   if (left <= 0) return;
   const StateView state = view_state(t.state[q], t.count[q]);
   T *first = (T*) t.m[q] + e, *second = (T*) t.v[q] + e;
-  const bool whole = left >= 4 && (((uintptr_t) first | (uintptr_t) second) & (4 * sizeof(T) - 1)) == 0;
-  const uint32_t codes_m = *(const uint32_t*) (state.m + e), codes_v = *(const uint32_t*) (state.v + e);
   const int exponent_m = state.exponents[2 * (e / kBlock)], exponent_v = state.exponents[2 * (e / kBlock) + 1];
-  float m[4], v[4];
+  const bool whole = left >= 4 * kWords && (((uintptr_t) first | (uintptr_t) second) & 15) == 0;
+  struct alignas(16) { T x[4 * kWords]; } pm, pv;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) decode(codes_m >> (8 * k), codes_v >> (8 * k), exponent_m, exponent_v, m[k], v[k]);
-  store4(first, left, whole, m), store4(second, left, whole, v);
+  for (int w = 0; w < kWords; ++w) {
+    float m[4], v[4];
+    decode4(*(const uint32_t*) (state.m + e + 4 * w), *(const uint32_t*) (state.v + e + 4 * w), exponent_m, exponent_v, m, v);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) pm.x[4 * w + k] = from_float<T>(m[k]), pv.x[4 * w + k] = from_float<T>(v[k]);
+  }
+  if (whole) {
+    *(decltype(pm)*) first = pm, *(decltype(pv)*) second = pv;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4 * kWords; ++k)
+      if (k < left) first[k] = pm.x[k], second[k] = pv.x[k];
+  }
 }
 
 // 8-bit moments of given values (m, v), rounded to the nearest: they are taken over once, not step after step.
@@ -470,11 +496,11 @@ int adamw_update(const char* what, int bits, int n, int dtype, const int64_t* co
 }
 
 int moments(const char* what, int n, const int64_t* count, const void* const* state, const void* const* m, const void* const* v,
-            size_t size, MomentsTable& t) {
+            size_t size, int64_t per_block, MomentsTable& t) {
   FSGS_REQUIRE(n >= 0 && n <= kMaxTensors, "%s: at most %d tensors", what, kMaxTensors);
   if (n == 0) return kOk;
   FSGS_REQUIRE(count && state && m && v, "%s: null pointer", what);
-  if (const int rc = lay_out(what, t, t.first_block, n, count, 1024)) return rc;
+  if (const int rc = lay_out(what, t, t.first_block, n, count, per_block)) return rc;
   for (int q = 0; q < n; ++q) {
     FSGS_REQUIRE(count[q] == 0 || (state[q] && m[q] && v[q] && (uintptr_t) state[q] % 4 == 0 &&
                                    ((uintptr_t) m[q] | (uintptr_t) v[q]) % size == 0), "%s: bad tensor %d", what, q);
@@ -504,7 +530,7 @@ FSGS_API int fsgs_adamw8_unpack_multi(int n_tensors, int dtype, const int64_t* c
   const char* what = "adamw8_moments";
   FSGS_REQUIRE(is_type(dtype), "%s: element type not supported", what);
   MomentsTable t{};
-  if (const int rc = moments(what, n_tensors, count, state, m, v, type_size(dtype), t)) return rc;
+  if (const int rc = moments(what, n_tensors, count, state, m, v, type_size(dtype), 4096 / type_size(dtype), t)) return rc;
   if (t.first_block[t.n] == 0) return kOk;
   auto kernel = dtype == kFloat32 ? adamw8_unpack_kernel<float> : dtype == kFloat16 ? adamw8_unpack_kernel<__half> : adamw8_unpack_kernel<__hip_bfloat16>;
   hipLaunchKernelGGL(kernel, dim3(t.first_block[t.n]), dim3(256), 0, (hipStream_t) stream, t);
@@ -515,7 +541,7 @@ FSGS_API int fsgs_adamw8_pack_multi(int n_tensors, const int64_t* count, const f
                                     void* const* state, void* stream) {
   const char* what = "adamw8_pack";
   MomentsTable t{};
-  if (const int rc = moments(what, n_tensors, count, state, (const void* const*) m, (const void* const*) v, 4, t)) return rc;
+  if (const int rc = moments(what, n_tensors, count, state, (const void* const*) m, (const void* const*) v, 4, 1024, t)) return rc;
   if (t.first_block[t.n] == 0) return kOk;
   hipLaunchKernelGGL(adamw8_pack_kernel, dim3(t.first_block[t.n]), dim3(256), 0, (hipStream_t) stream, t);
   return check_launch(what);

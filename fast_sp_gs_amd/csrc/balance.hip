@@ -23,12 +23,18 @@ namespace fsgs {
 namespace {
 
 constexpr int kMostChoices   = 64;
-constexpr int kPassBlocks    = 1024;  // of the pass over logits
+constexpr int kRowBlocks     = 512;   // of the pass over logits
+// threads of its blocks: with 64 values in each lane a wavefront has the registers of a SIMD to itself
+constexpr int row_threads(int vals) { return vals == 64 ? 256 : 512; }
 constexpr int kMostInLanes   = 4096;  // superpoints whose row is held by the lanes of one wavefront
 constexpr int kNeighbourBlocks = 256;
 constexpr int kNeighbourThreads = 1024;
 constexpr int kMostInLds     = 5400;  // superpoints whose sums (8 bytes) and counts (4) of a block fit in 64 KB beside a few words
+constexpr int kSlopeThreads  = 512;   // of their backward
+constexpr int kSlopeBlocks   = 1024;
+constexpr int kMostSlopes    = 8192;  // that it keeps in LDS
 constexpr float kLog2e       = 1.44269504f;
+constexpr float kLowest      = -3.402823466e38f;
 
 // What a block of a pass leaves: sums and counts of every superpoint, the rows that counted, whether something was no weight or no index.
 struct BlockRows {
@@ -46,44 +52,47 @@ struct alignas(n * sizeof(T)) Pack {
   T x[n];
 };
 
-// ---- reductions over the kLanes lanes of a row; every one of them gets the result ----------------------------------------------
-template <int kCtrl>
-__device__ __forceinline__ uint32_t moved(uint32_t x) {
-  return (uint32_t) __builtin_amdgcn_update_dpp(0, (int) x, kCtrl, 0xf, 0xf, true);
-}
 __device__ __forceinline__ float as_float(uint32_t x) { return __builtin_bit_cast(float, x); }
 __device__ __forceinline__ uint32_t as_uint(float x) { return __builtin_bit_cast(uint32_t, x); }
+
+// ---- reductions over the kLanes lanes of a row; every one of them gets the result ----------------------------------------------
+template <int kCtrl>
+__device__ __forceinline__ int moved(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, kCtrl, 0xf, 0xf, true);
+}
 template <int kLanes, typename F>
-__device__ __forceinline__ uint32_t over_lanes(uint32_t x, F f) {
-  x = f(x, moved<0xB1>(x)), x = f(x, moved<0x4E>(x));                         // quad_perm: neighbours, then pairs of them
-  if (kLanes >= 16) x = f(x, moved<0x141>(x)), x = f(x, moved<0x140>(x));     // row_half_mirror, row_mirror
+__device__ __forceinline__ int over_lanes(int x, F f) {
+  x = f(x, moved<0xB1>(x)), x = f(x, moved<0x4E>(x));  // quad_perm: neighbours, then pairs of them
+  if (kLanes >= 8) x = f(x, moved<0x141>(x));          // row_half_mirror
+  if (kLanes >= 16) x = f(x, moved<0x140>(x));         // row_mirror
   if (kLanes == 64) {
-    const uint32_t a = f(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16));
-    const uint32_t b = f(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48));
+    const int a = f(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16));
+    const int b = f(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48));
     x = f(a, b);
   }
   return x;
 }
 template <int kLanes>
-__device__ __forceinline__ float row_max(float x) {
-  return as_float(over_lanes<kLanes>(as_uint(x), [](uint32_t a, uint32_t b) { return as_uint(fmaxf(as_float(a), as_float(b))); }));
+__device__ __forceinline__ int row_max(int x) {
+  return over_lanes<kLanes>(x, [](int a, int b) { return max(a, b); });
+}
+template <int kLanes>
+__device__ __forceinline__ int row_min(int x) {
+  return over_lanes<kLanes>(x, [](int a, int b) { return min(a, b); });
+}
+template <int kLanes>
+__device__ __forceinline__ int row_count(int x) {
+  return over_lanes<kLanes>(x, [](int a, int b) { return a + b; });
 }
 template <int kLanes>
 __device__ __forceinline__ float row_sum(float x) {
-  return as_float(over_lanes<kLanes>(as_uint(x), [](uint32_t a, uint32_t b) { return as_uint(as_float(a) + as_float(b)); }));
+  return as_float(over_lanes<kLanes>((int) as_uint(x), [](int a, int b) { return (int) as_uint(as_float(a) + as_float(b)); }));
 }
-template <int kLanes>
-__device__ __forceinline__ uint32_t row_umax(uint32_t x) {
-  return over_lanes<kLanes>(x, [](uint32_t a, uint32_t b) { return max(a, b); });
-}
-template <int kLanes>
-__device__ __forceinline__ uint32_t row_umin(uint32_t x) {
-  return over_lanes<kLanes>(x, [](uint32_t a, uint32_t b) { return min(a, b); });
-}
-template <int kLanes>
-__device__ __forceinline__ uint32_t row_count(uint32_t x) {
-  return over_lanes<kLanes>(x, [](uint32_t a, uint32_t b) { return a + b; });
-}
+// Floats as integers of the same order (-0 directly below 0): their maximum takes one instruction with a lane's exchange, where that
+// of floats quiets its operands first. It is its own inverse.
+__device__ __forceinline__ int ordered(int bits) { return bits ^ ((bits >> 31) & 0x7fffffff); }
+__device__ __forceinline__ int ordered(float x) { return ordered((int) as_uint(x)); }
+__device__ __forceinline__ float unordered(int x) { return as_float((uint32_t) ordered(x)); }
 
 // ---- rows of logits in the lanes of a wavefront ------------------------------------------------------------------------------------
 // kLanes lanes have a row, kVals of its columns each, in pieces of 16 bytes: piece i of lane l begins at column (i kLanes + l) 16 / size.
@@ -92,120 +101,167 @@ __device__ __forceinline__ int column(int lane, int j) {
   constexpr int kPiece = 16 / sizeof(T);
   return (j / kPiece * kLanes + lane) * kPiece + j % kPiece;
 }
-// Columns that there are not read as -inf. `whole`: pieces are aligned, and end where the row ends.
+// A lane's part of a row as it lies in memory. A row that is not `on` is read where the first one is, a column that there is not where the
+// row begins: no branch stands between the loads, so that they stay in flight while the row before is worked on.
 template <typename T, int kLanes, int kVals>
-__device__ __forceinline__ void load_row(const T* __restrict__ row, int M, bool whole, int lane, float x[kVals]) {
-  constexpr int kPiece = 16 / sizeof(T);
+struct Row {
+  static constexpr int kPiece = 16 / sizeof(T);
+  Pack<T, kPiece> piece[kVals / kPiece];
+
+  template <bool kWhole>  // pieces are aligned, and end where the row ends
+  __device__ __forceinline__ void load(const T* __restrict__ row, int M, int lane) {
 #pragma unroll
-  for (int j = 0; j < kVals; j += kPiece) {
-    const int c = column<T, kLanes>(lane, j);
-    if (whole) {
-      if (c < M) {
-        const Pack<T, kPiece> q = *(const Pack<T, kPiece>*) (row + c);
+    for (int i = 0; i < kVals / kPiece; ++i) {
+      const int c = column<T, kLanes>(lane, i * kPiece);
+      if (kWhole) piece[i] = *(const Pack<T, kPiece>*) (row + (c < M ? c : 0));
+      else
 #pragma unroll
-        for (int k = 0; k < kPiece; ++k) x[j + k] = to_float(q.x[k]);
-      } else {
+        for (int k = 0; k < kPiece; ++k) piece[i].x[k] = row[c + k < M ? c + k : 0];
+    }
+  }
+  // -inf for what there is not; `full`: every lane has kVals columns
+  __device__ __forceinline__ void values(float x[kVals], int M, bool full, bool on, int lane) const {
 #pragma unroll
-        for (int k = 0; k < kPiece; ++k) x[j + k] = -INFINITY;
+    for (int j = 0; j < kVals; ++j) x[j] = to_float(piece[j / kPiece].x[j % kPiece]);
+    if (wave_ballot(!on) || !full) {
+      const int there = on ? M : 0, l = keep_local(lane);
+#pragma unroll
+      for (int j = 0; j < kVals; ++j) x[j] = column<T, kLanes>(l, j) < there ? x[j] : -INFINITY;
+    }
+  }
+};
+
+// How many values of the row reach t. A row that has the wavefront to itself is counted by the comparisons' lane masks.
+template <int kLanes, int kVals>
+__device__ __forceinline__ int reaching(const float x[kVals], float t) {
+  int n = 0;
+#pragma unroll
+  for (int j = 0; j < kVals; ++j) n += kLanes == 64 ? (int) __popcll(wave_ballot(x[j] >= t)) : x[j] >= t ? 1 : 0;
+  return kLanes == 64 ? n : row_count<kLanes>(n);
+}
+
+// Counts the row's K largest values above -inf, the lowest column first among equals. `lane_top`: the largest of the lane, `top` of the row,
+// ordered. The K-th largest of the lanes' own largest is reached by at least K values, and mostly by no other: 4 of 512 values lie
+// in 4 of 64 lanes in 9 rows of 10. Otherwise the threshold rises value by value, after a walk down from the top where that is nearer.
+template <typename T, int kLanes, int kVals>
+__device__ __forceinline__ void choose(const float x[kVals], int lane_top, int top, int K, int lane, int count[kVals]) {
+  const int lowest = ordered(-INFINITY);
+  int t_ordered = top;
+  for (int r = 1; r < K; ++r) t_ordered = row_max<kLanes>(lane_top < t_ordered ? lane_top : lowest);
+  float t = unordered(max(t_ordered, ordered(kLowest)));
+  int n = reaching<kLanes, kVals>(x, t);
+  if (wave_ballot(n > K)) {
+    if (wave_ballot(n > 2 * K)) {
+      float s = unordered(top);
+      for (int r = 1; r < K; ++r) {
+        float below = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kVals; ++j) below = fmaxf(below, x[j] < s ? x[j] : -INFINITY);
+        s = unordered(row_max<kLanes>(ordered(below)));
       }
-    } else {
+      s = fmaxf(s, kLowest);
+      const int m = reaching<kLanes, kVals>(x, s);
+      if (n > 2 * K) t = s, n = m;
+    }
+    for (;;) {
+      float above = INFINITY;
 #pragma unroll
-      for (int k = 0; k < kPiece; ++k) x[j + k] = c + k < M ? to_float(row[c + k]) : -INFINITY;
+      for (int j = 0; j < kVals; ++j) above = fminf(above, x[j] > t ? x[j] : INFINITY);
+      above = unordered(row_min<kLanes>(ordered(above)));
+      const int m = reaching<kLanes, kVals>(x, above);
+      const bool better = n > K && m >= K && above > t;
+      if (better) t = above, n = m;
+      if (!wave_ballot(better)) break;
+    }
+    const bool ties = n > K;  // of values equal to t
+    if (wave_ballot(ties)) {
+      int greater = 0;
+#pragma unroll
+      for (int j = 0; j < kVals; ++j) {
+        greater += x[j] > t ? 1 : 0;
+        count[j] += (ties ? x[j] > t : x[j] >= t) ? 1 : 0;
+      }
+      greater = row_count<kLanes>(greater);
+      int left = ties ? K - greater : 0, at = -1;
+      while (wave_ballot(left > 0)) {
+        const int l = keep_local(lane);  // or every column's index stays in a register of its own
+        int where = 0x7fffffff;
+#pragma unroll
+        for (int j = 0; j < kVals; ++j) {
+          const int c = column<T, kLanes>(l, j);
+          where = min(where, x[j] == t && c > at ? c : 0x7fffffff);
+        }
+        at = row_min<kLanes>(where);
+#pragma unroll
+        for (int j = 0; j < kVals; ++j) count[j] += left > 0 && column<T, kLanes>(l, j) == at ? 1 : 0;
+        --left;
+      }
+      return;
     }
   }
+#pragma unroll
+  for (int j = 0; j < kVals; ++j) count[j] += x[j] >= t ? 1 : 0;
 }
 
-// Counts the row's K largest values. `top`: the largest. First the K-th largest of the distinct values, K - 1 passes over registers;
-// if no more than K values reach it these are the ones. Otherwise some are equal, and they are taken one by one in order
-// of (value falling, column rising).
-template <typename T, int kLanes, int kVals>
-__device__ __forceinline__ void choose(const float x[kVals], float top, int K, int lane, int count[kVals]) {
-  float t = top;
-  for (int r = 1; r < K; ++r) {
-    float next = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < kVals; ++j) next = fmaxf(next, x[j] < t ? x[j] : -INFINITY);
-    t = row_max<kLanes>(next);
-  }
-  const float least = fmaxf(t, -3.402823466e38f);  // -inf is not chosen
-  uint32_t n = 0;
-#pragma unroll
-  for (int j = 0; j < kVals; ++j) n += x[j] >= least ? 1 : 0;
-  const bool more = row_count<kLanes>(n) > (uint32_t) K;
-  if (!wave_ballot(more)) {
-#pragma unroll
-    for (int j = 0; j < kVals; ++j) count[j] += x[j] >= least ? 1 : 0;
-    return;
-  }
-  float value = INFINITY;
-  uint32_t at = 0xffffffffu;  // the last one taken: before all
-  bool first = true;
-  for (int r = 0; r < K; ++r) {
-    float best = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < kVals; ++j) {
-      const bool after = first || x[j] < value || (x[j] == value && (uint32_t) column<T, kLanes>(lane, j) > at);
-      best = fmaxf(best, after ? x[j] : -INFINITY);
-    }
-    best = row_max<kLanes>(best);
-    uint32_t where = 0xffffffffu;
-#pragma unroll
-    for (int j = 0; j < kVals; ++j) {
-      const uint32_t c = (uint32_t) column<T, kLanes>(lane, j);
-      if (x[j] == best && (first || best < value || c > at)) where = min(where, c);
-    }
-    where = row_umin<kLanes>(where);
-    if (best > -INFINITY)
-#pragma unroll
-      for (int j = 0; j < kVals; ++j) count[j] += (uint32_t) column<T, kLanes>(lane, j) == where ? 1 : 0;
-    value = best, at = where, first = false;
-  }
-}
-
-template <typename T, int kLanes, int kVals>
-__global__ void __launch_bounds__(256) balance_rows_kernel(int64_t N, int M, int64_t ld, int K, const T* __restrict__ logits,
-    const uint8_t* __restrict__ rows, float2* __restrict__ stats, float* __restrict__ sums, int* __restrict__ counts,
-    BlockRows* __restrict__ blocks, unsigned* __restrict__ ticket) {
-  constexpr int kRows = 64 / kLanes;  // of a wavefront
+template <typename T, int kLanes, int kVals, bool kWhole>
+__global__ void __launch_bounds__(row_threads(kVals)) balance_rows_kernel(int64_t N, int M, int64_t ld, int K,
+    const T* __restrict__ logits, const uint8_t* __restrict__ rows, float2* __restrict__ stats, float* __restrict__ sums,
+    int* __restrict__ counts, BlockRows* __restrict__ blocks, unsigned* __restrict__ ticket) {
+  constexpr int kRows = 64 / kLanes, kThreads = row_threads(kVals), kWaves = kThreads / 64;
   __shared__ float s_sum[kLanes * kVals];
   __shared__ int s_count[kLanes * kVals];
-  __shared__ int s_rows[4];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & (kLanes - 1), group = (threadIdx.x & 63) / kLanes;
-  const bool whole = M % (16 / sizeof(T)) == 0 && ld * sizeof(T) % 16 == 0 && ((uintptr_t) logits & 15) == 0;
+  __shared__ int s_rows[kWaves];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & (kLanes - 1);
+  const int group = kLanes == 64 ? 0 : (threadIdx.x & 63) / kLanes;
+  const bool full = M == kLanes * kVals;
   float sum[kVals];
   int count[kVals], counted = 0;
 #pragma unroll
   for (int j = 0; j < kVals; ++j) sum[j] = 0.0f, count[j] = 0;
-  const int64_t step = (int64_t) gridDim.x * 4 * kRows;
-  for (int64_t base = ((int64_t) blockIdx.x * 4 + wave) * kRows; base < N; base += step) {
-    const int64_t row = base + group;
-    const bool on = row < N && (!rows || rows[row]);
+  const int64_t step = (int64_t) gridDim.x * kWaves * kRows;
+  int64_t base = ((int64_t) blockIdx.x * kWaves + wave) * kRows;
+
+  // whether a row counts is known a row before its values are asked for, those a row before they are worked on
+  auto mask_of = [&](int64_t row) { return rows ? (int) rows[row < N ? row : 0] : 1; };
+  auto on_of = [&](int64_t row, int mask) { return row < N && mask != 0; };
+  auto address = [&](int64_t row, bool on) { return logits + (on ? row : 0) * ld; };
+  auto work = [&](const Row<T, kLanes, kVals>& row, int64_t at, bool on) {
     float x[kVals];
-    if (on) {
-      load_row<T, kLanes, kVals>(logits + row * ld, M, whole, lane, x);
-    } else {
+    row.values(x, M, full, on, lane);
+    float lane_top = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < kVals; ++j) x[j] = -INFINITY;
-    }
-    float top = x[0];
-#pragma unroll
-    for (int j = 1; j < kVals; ++j) top = fmaxf(top, x[j]);
-    top = row_max<kLanes>(top);
-    choose<T, kLanes, kVals>(x, top, K, lane, count);
+    for (int j = 0; j < kVals; ++j) lane_top = fmaxf(lane_top, x[j]);
+    const int lane_top_ordered = ordered(lane_top), top_ordered = row_max<kLanes>(lane_top_ordered);
+    choose<T, kLanes, kVals>(x, lane_top_ordered, top_ordered, K, lane, count);
     // a row without a number (top is -inf): the sum is 0, or NaN where one of its values is, which counts
-    const float shift = top == -INFINITY ? 0.0f : top;
+    const float top = unordered(top_ordered), shift = top == -INFINITY ? 0.0f : top;
     float total = 0.0f;
 #pragma unroll
     for (int j = 0; j < kVals; ++j) x[j] = __builtin_amdgcn_exp2f((x[j] - shift) * kLog2e), total += x[j];
     total = row_sum<kLanes>(total);
     const bool counts_in = !(total == 0.0f);
-    const float scale = counts_in ? 1.0f / total : 0.0f;
+    const float scale = counts_in ? __builtin_amdgcn_rcpf(total) : 0.0f;
 #pragma unroll
     for (int j = 0; j < kVals; ++j) sum[j] = fmaf(x[j], scale, sum[j]);
-    if (lane == 0 && row < N) {
-      if (stats) stats[row] = make_float2(shift, scale);
+    if (lane == 0 && at < N) {
+      if (stats) stats[at] = make_float2(shift, scale);
       counted += counts_in ? 1 : 0;
     }
+  };
+  Row<T, kLanes, kVals> a, b;
+  bool on_a = on_of(base + group, mask_of(base + group)), on_b;
+  int mask = mask_of(base + step + group);
+  a.template load<kWhole>(address(base + group, on_a), M, lane);
+  for (; base < N; base += 2 * step) {
+    const int64_t at = base + group;
+    on_b = on_of(at + step, mask);
+    mask = mask_of(at + 2 * step);
+    b.template load<kWhole>(address(at + step, on_b), M, lane);
+    work(a, at, on_a);
+    on_a = on_of(at + 2 * step, mask);
+    mask = mask_of(at + 3 * step);
+    a.template load<kWhole>(address(at + 2 * step, on_a), M, lane);
+    if (base + step < N) work(b, at + step, on_b);
   }
   // the rows' groups of a wavefront, then the wavefronts one after the other
 #pragma unroll
@@ -215,7 +271,7 @@ __global__ void __launch_bounds__(256) balance_rows_kernel(int64_t N, int M, int
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) counted += __shfl_xor(counted, d);
   if ((threadIdx.x & 63) == 0) s_rows[wave] = counted;
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < kWaves; ++w) {
     if (w == wave && group == 0)
 #pragma unroll
       for (int j = 0; j < kVals; ++j) {
@@ -224,59 +280,59 @@ __global__ void __launch_bounds__(256) balance_rows_kernel(int64_t N, int M, int
       }
     __syncthreads();
   }
-  for (int c = threadIdx.x; c < M; c += 256) {
+  for (int c = threadIdx.x; c < M; c += kThreads)
     sums[(size_t) blockIdx.x * M + c] = s_sum[c], counts[(size_t) blockIdx.x * M + c] = s_count[c];
-  }
   if (threadIdx.x == 0) {
-    blocks[blockIdx.x] = BlockRows{s_rows[0] + s_rows[1] + s_rows[2] + s_rows[3], 0};
+    int all = 0;
+    for (int w = 0; w < kWaves; ++w) all += s_rows[w];
+    blocks[blockIdx.x] = BlockRows{all, 0};
     if (blockIdx.x == 0) *ticket = 0;
   }
 }
 
-template <typename T, int kLanes, int kVals>
+// kWhole: also of the gradient's rows
+template <typename T, int kLanes, int kVals, bool kWhole>
 __global__ void __launch_bounds__(256) balance_rows_backward_kernel(int64_t N, int M, int64_t ld, const T* __restrict__ logits,
     const float2* __restrict__ stats, const int* __restrict__ counts, const int64_t* __restrict__ totals,
     const float* __restrict__ g_loss, const float* __restrict__ g_importance, T* __restrict__ grad) {
   constexpr int kRows = 64 / kLanes, kPiece = 16 / sizeof(T);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & (kLanes - 1), group = (threadIdx.x & 63) / kLanes;
-  const bool whole = M % kPiece == 0 && ld * sizeof(T) % 16 == 0 && ((uintptr_t) logits & 15) == 0;
-  const bool whole_out = M % kPiece == 0 && ((uintptr_t) grad & 15) == 0;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & (kLanes - 1);
+  const int group = kLanes == 64 ? 0 : (threadIdx.x & 63) / kLanes;
+  const bool full = M == kLanes * kVals;
   const float rows = (float) max(totals[1], (int64_t) 1);
   const float of_counts = g_loss ? *g_loss * (float) M / (float) max(totals[0], (int64_t) 1) / rows : 0.0f;
-  float a[kVals];
+  float slope[kVals];
 #pragma unroll
   for (int j = 0; j < kVals; ++j) {
     const int c = column<T, kLanes>(lane, j);
-    a[j] = c < M ? of_counts * (float) counts[c] + (g_importance ? g_importance[c] / rows : 0.0f) : 0.0f;
+    slope[j] = c < M ? of_counts * (float) counts[c] + (g_importance ? g_importance[c] / rows : 0.0f) : 0.0f;
   }
   const int64_t step = (int64_t) gridDim.x * 4 * kRows;
-  for (int64_t base = ((int64_t) blockIdx.x * 4 + wave) * kRows; base < N; base += step) {
-    const int64_t row = base + group;
-    const float2 stat = row < N ? stats[row] : make_float2(0.0f, 0.0f);
-    const bool on = !(stat.y == 0.0f);  // a row that counted
-    float x[kVals];
-    if (on) {
-      load_row<T, kLanes, kVals>(logits + row * ld, M, whole, lane, x);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kVals; ++j) x[j] = -INFINITY;
-    }
-    float mean = 0.0f;
+  int64_t base = ((int64_t) blockIdx.x * 4 + wave) * kRows;
+
+  // y is 0 in rows that did not count: they are not read
+  auto stat_of = [&](int64_t row) { return stats[row < N ? row : 0]; };
+  auto on_of = [&](int64_t row, float2 stat) { return row < N && !(stat.y == 0.0f); };
+  auto address = [&](int64_t row, bool on) { return logits + (on ? row : 0) * ld; };
+  auto work = [&](const Row<T, kLanes, kVals>& row, int64_t at, float2 stat) {
+    const bool on = on_of(at, stat);
+    float x[kVals], mean = 0.0f;
+    row.values(x, M, full, on, lane);
 #pragma unroll
     for (int j = 0; j < kVals; ++j) {
       x[j] = __builtin_amdgcn_exp2f((x[j] - stat.x) * kLog2e) * stat.y;
-      mean = fmaf(x[j], a[j], mean);
+      mean = fmaf(x[j], slope[j], mean);
     }
     mean = row_sum<kLanes>(mean);
-    if (row >= N) continue;
-    T* out = grad + row * M;
+    if (at >= N) return;
+    T* out = grad + at * M;
 #pragma unroll
     for (int j = 0; j < kVals; j += kPiece) {
       const int c = column<T, kLanes>(lane, j);
       Pack<T, kPiece> q;
 #pragma unroll
-      for (int k = 0; k < kPiece; ++k) from_float(x[j + k] * (a[j + k] - mean), q.x[k]);
-      if (whole_out) {
+      for (int k = 0; k < kPiece; ++k) from_float(x[j + k] * (slope[j + k] - mean), q.x[k]);
+      if (kWhole) {
         if (c < M) *(Pack<T, kPiece>*) (out + c) = q;
       } else {
 #pragma unroll
@@ -284,6 +340,19 @@ __global__ void __launch_bounds__(256) balance_rows_backward_kernel(int64_t N, i
           if (c + k < M) out[c + k] = q.x[k];
       }
     }
+  };
+  Row<T, kLanes, kVals> a, b;
+  float2 stat_a = stat_of(base + group), stat_b = stat_of(base + step + group), after;
+  a.template load<kWhole>(address(base + group, on_of(base + group, stat_a)), M, lane);
+  for (; base < N; base += 2 * step) {
+    const int64_t at = base + group;
+    after = stat_of(at + 2 * step);
+    b.template load<kWhole>(address(at + step, on_of(at + step, stat_b)), M, lane);
+    work(a, at, stat_a);
+    stat_a = after, after = stat_of(at + 3 * step);
+    a.template load<kWhole>(address(at + 2 * step, on_of(at + 2 * step, stat_a)), M, lane);
+    if (base + step < N) work(b, at + step, stat_b);
+    stat_b = after;
   }
 }
 
@@ -383,7 +452,9 @@ __global__ void __launch_bounds__(256) balance_wide_backward_kernel(int64_t N, i
 // or an index that is none, is reported and left out.
 constexpr float kWeightUnits = 2147483648.0f;
 
-template <bool kLds>
+// A thread takes a row, four neighbours at a time: all loads of four are on their way before the first is looked at. kQuads: K is a
+// multiple of four and the addresses allow 16 bytes.
+template <bool kLds, bool kQuads>
 __global__ void __launch_bounds__(kNeighbourThreads) balance_neighbours_kernel(int64_t N, int M, int K,
     const float* __restrict__ weights, const int64_t* __restrict__ indices, const uint8_t* __restrict__ rows,
     unsigned long long* __restrict__ sums, int* __restrict__ counts, BlockRows* __restrict__ blocks, unsigned* __restrict__ ticket) {
@@ -400,16 +471,35 @@ __global__ void __launch_bounds__(kNeighbourThreads) balance_neighbours_kernel(i
     if (rows && !rows[n]) continue;
     ++counted;
     float best = -1.0f;
-    int64_t where = 0;
-    for (int k = 0; k < K; ++k) {
-      const float w = weights[n * K + k];
-      const int64_t m = indices[n * K + k];
-      if (!(w >= 0.0f && w <= 1.0001f) || m < 0 || m >= M) {
-        invalid = 1;
-        continue;
+    int where = 0;
+    const float* row_w     = weights + n * K;
+    const int64_t* row_i = indices + n * K;
+    for (int k = 0; k < K; k += 4) {
+      float w[4];
+      int64_t m[4];
+      if (kQuads) {
+        const float4 q = *(const float4*) (row_w + k);
+        const longlong2 i = *(const longlong2*) (row_i + k), j = *(const longlong2*) (row_i + k + 2);
+        w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+        m[0] = i.x, m[1] = i.y, m[2] = j.x, m[3] = j.y;
+      } else {
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const int at = min(k + d, K - 1);
+          w[d] = row_w[at], m[d] = row_i[at];
+        }
       }
-      atomicAdd(&sum[m], (unsigned long long) (uint32_t) __float2uint_rn(w * kWeightUnits));
-      if (w > best) best = w, where = m;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        if (!kQuads && k + d >= K) continue;
+        const bool valid = w[d] >= 0.0f && w[d] <= 1.0001f && (uint64_t) m[d] < (uint64_t) M;
+        if (!valid) {
+          invalid = 1;
+          continue;
+        }
+        atomicAdd(&sum[(int) m[d]], (unsigned long long) __float2uint_rn(w[d] * kWeightUnits));
+        if (w[d] > best) best = w[d], where = (int) m[d];
+      }
     }
     if (best >= 0.0f) atomicAdd(&count[where], 1);
   }
@@ -425,19 +515,62 @@ __global__ void __launch_bounds__(kNeighbourThreads) balance_neighbours_kernel(i
   }
 }
 
-__global__ void __launch_bounds__(256) balance_neighbours_backward_kernel(int64_t N, int M, int K, const int64_t* __restrict__ indices,
-    const uint8_t* __restrict__ rows, const int* __restrict__ counts, const int64_t* __restrict__ totals,
-    const float* __restrict__ g_loss, const float* __restrict__ g_importance, float* __restrict__ grad) {
+// A thread takes four pairs. kLds: the slopes of all superpoints lie in LDS, which answers 64 lanes' addresses at once where the cache
+// takes them line by line.
+template <bool kLds>
+__global__ void __launch_bounds__(kSlopeThreads) balance_neighbours_backward_kernel(int64_t N, int M, int K,
+    const int64_t* __restrict__ indices, const uint8_t* __restrict__ rows, const int* __restrict__ counts,
+    const int64_t* __restrict__ totals, const float* __restrict__ g_loss, const float* __restrict__ g_importance,
+    float* __restrict__ grad) {
+  extern __shared__ float s_slope[];
   const float of_rows = (float) max(totals[1], (int64_t) 1);
   const float of_counts = g_loss ? *g_loss * (float) M / (float) max(totals[0], (int64_t) 1) / of_rows : 0.0f;
-  for (int64_t e = (int64_t) blockIdx.x * 256 + threadIdx.x; e < N * K; e += (int64_t) gridDim.x * 256) {
-    float g = 0.0f;
-    if (!rows || rows[e / K]) {
-      const int64_t m = indices[e];
-      if (m < 0 || m >= M) g = __builtin_nanf("");
-      else g = of_counts * (float) counts[m] + (g_importance ? g_importance[m] / of_rows : 0.0f);
+  auto slope = [&](int m) { return of_counts * (float) counts[m] + (g_importance ? g_importance[m] / of_rows : 0.0f); };
+  if (kLds) {
+    for (int m = threadIdx.x; m < M; m += kSlopeThreads) s_slope[m] = slope(m);
+    __syncthreads();
+  }
+  const bool aligned = (((uintptr_t) indices | (uintptr_t) grad) & 15) == 0;
+  const double per_row = 1.0 / (double) K;
+  const int64_t pairs = N * K;
+  for (int64_t e = ((int64_t) blockIdx.x * kSlopeThreads + threadIdx.x) * 4; e < pairs; e += (int64_t) gridDim.x * kSlopeThreads * 4) {
+    const bool whole = aligned && e + 4 <= pairs;
+    int64_t m[4];
+    if (whole) {
+      const longlong2 i = *(const longlong2*) (indices + e), j = *(const longlong2*) (indices + e + 2);
+      m[0] = i.x, m[1] = i.y, m[2] = j.x, m[3] = j.y;
+    } else {
+#pragma unroll
+      for (int d = 0; d < 4; ++d) m[d] = indices[min(e + d, pairs - 1)];
     }
-    grad[e] = g;
+    bool on[4] = {true, true, true, true};
+    if (rows) {
+      // the row of the first pair: the product is off by one at most, pairs being fewer than 2^53
+      int64_t row = (int64_t) ((double) e * per_row);
+      int k = (int) (e - row * K);
+      if (k < 0) --row, k += K;
+      if (k >= K) ++row, k -= K;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        on[d] = rows[min(row, N - 1)] != 0;
+        if (++k == K) k = 0, ++row;
+      }
+    }
+    float g[4];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      const bool valid = (uint64_t) m[d] < (uint64_t) M;
+      const int at = valid && on[d] ? (int) m[d] : 0;
+      const float a = kLds ? s_slope[at] : slope(at);
+      g[d] = !on[d] ? 0.0f : valid ? a : __builtin_nanf("");
+    }
+    if (whole) {
+      *(float4*) (grad + e) = make_float4(g[0], g[1], g[2], g[3]);
+    } else {
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+        if (e + d < pairs) grad[e + d] = g[d];
+    }
   }
 }
 
@@ -447,7 +580,8 @@ __global__ void __launch_bounds__(256) clear_kernel(int M, unsigned long long* s
 }
 
 // ---- the blocks' sums together -----------------------------------------------------------------------------------------------------------
-// A block takes 32 superpoints, 32 threads of it a superpoint's blocks in turn; the last block to end forms the loss of all of them.
+// A block takes 16 superpoints, 64 threads of it a superpoint's blocks in turn; the last block to end forms the loss of all of them.
+constexpr int kTotalColumns = 16;
 __device__ __forceinline__ double value_of(float s) { return (double) s; }
 __device__ __forceinline__ double value_of(unsigned long long s) { return (double) s * (1.0 / kWeightUnits); }
 __device__ __forceinline__ double added(double a, float s) { return a + (double) s; }
@@ -461,34 +595,40 @@ __global__ void __launch_bounds__(1024) balance_totals_kernel(int G, int G_rows,
     const int* __restrict__ block_counts, const BlockRows* __restrict__ blocks, double* __restrict__ parts, unsigned* __restrict__ ticket,
     float* __restrict__ loss, int* __restrict__ counts, float* __restrict__ importance, int64_t* __restrict__ totals) {
   using Total = typename TotalOf<S>::type;
-  __shared__ Total s_sum[32][33];
-  __shared__ int s_count[32][33];
-  __shared__ int s_rows, s_invalid, s_last;
-  const int c = threadIdx.x & 31, slice = threadIdx.x >> 5, m = blockIdx.x * 32 + c;
-  if (threadIdx.x == 0) s_rows = 0, s_invalid = 0;
+  constexpr int kSlices = 1024 / kTotalColumns, kWaves = 16;
+  static_assert(kTotalColumns == 16 && kSlices == 4 * kWaves, "a wavefront has four slices of 16 columns");
+  __shared__ Total s_sum[kWaves][kTotalColumns];
+  __shared__ int s_count[kWaves][kTotalColumns], s_rows[kWaves], s_invalid[kWaves], s_last;
+  const int c = threadIdx.x % kTotalColumns, slice = threadIdx.x / kTotalColumns, m = blockIdx.x * kTotalColumns + c;
+  const int wave = threadIdx.x >> 6;
+  int rows = 0, invalid = 0, count = 0;
+  for (int g = threadIdx.x; g < G_rows; g += 1024) rows += blocks[g].counted, invalid |= blocks[g].invalid;
   Total sum = 0;
-  int count = 0;
   if (m < M)
 #pragma unroll 8
-    for (int g = slice; g < G; g += 32) sum = added(sum, sums[(size_t) g * M + m]), count += block_counts[(size_t) g * M + m];
-  s_sum[slice][c] = sum, s_count[slice][c] = count;
+    for (int g = slice; g < G; g += kSlices) sum = added(sum, sums[(size_t) g * M + m]), count += block_counts[(size_t) g * M + m];
+  // in a fixed order: the slices of a wavefront, then the wavefronts
+#pragma unroll
+  for (int d = 16; d < 64; d <<= 1) sum += __shfl_xor(sum, d), count += __shfl_xor(count, d);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) rows += __shfl_xor(rows, d), invalid |= __shfl_xor(invalid, d);
+  if ((threadIdx.x & 63) < kTotalColumns) s_sum[wave][c] = sum, s_count[wave][c] = count;
+  if ((threadIdx.x & 63) == 0) s_rows[wave] = rows, s_invalid[wave] = invalid;
   __syncthreads();
-  for (int g = threadIdx.x; g < G_rows; g += 1024) {
-    atomicAdd(&s_rows, blocks[g].counted);
-    if (blocks[g].invalid) s_invalid = 1;
-  }
-  __syncthreads();
-  const int T = s_rows, of = max(T, 1);
-  if (threadIdx.x < 64) {  // a wavefront: the slices in order, then the block's share of the loss
+  int T = 0, any_invalid = 0;
+  for (int w = 0; w < kWaves; ++w) T += s_rows[w], any_invalid |= s_invalid[w];
+  const int of = max(T, 1);
+  if (wave == 0) {  // the block's share of the loss
     double chosen = 0.0, both = 0.0;
     if (slice == 0 && m < M) {
-      for (int k = 1; k < 32; ++k) sum += s_sum[k][c], count += s_count[k][c];
-      const double s = s_invalid ? __builtin_nan("") : value_of(sum);
+      sum = 0, count = 0;
+      for (int w = 0; w < kWaves; ++w) sum += s_sum[w][c], count += s_count[w][c];
+      const double s = any_invalid ? __builtin_nan("") : value_of(sum);
       counts[m] = count, importance[m] = (float) (s / of);
-      chosen = (double) count, both = (double) count * s;
+      chosen = (double) count, both = chosen * s;
     }
 #pragma unroll
-    for (int d = 16; d; d >>= 1) chosen += __shfl_xor(chosen, d), both += __shfl_xor(both, d);
+    for (int d = kTotalColumns / 2; d; d >>= 1) chosen += __shfl_xor(chosen, d), both += __shfl_xor(both, d);
     if (threadIdx.x == 0) {
       parts[2 * blockIdx.x] = chosen, parts[2 * blockIdx.x + 1] = both;
       __threadfence();
@@ -496,7 +636,7 @@ __global__ void __launch_bounds__(1024) balance_totals_kernel(int G, int G_rows,
     }
   }
   __syncthreads();
-  if (!s_last || threadIdx.x >= 64) return;
+  if (!s_last || wave != 0) return;
   __threadfence();
   double chosen = 0.0, both = 0.0;
   for (int b = threadIdx.x; b < (int) gridDim.x; b += 64)
@@ -516,18 +656,18 @@ struct Workspace {
     counts = align_up((size_t) G * M * sum_bytes, 256);
     blocks = counts + align_up((size_t) G * M * 4, 256);
     parts  = blocks + align_up((size_t) G_rows * sizeof(BlockRows), 256);
-    ticket = parts + align_up((size_t) div_up(M, 32) * 16, 256);
+    ticket = parts + align_up((size_t) div_up(M, kTotalColumns) * 16, 256);
     bytes  = ticket + 256;
   }
 };
 
-// Lanes a row, by its bytes: the fewest of 4, 16 and 64 that hold it in 32 values each (16 values for 4 lanes).
-int lanes_of(int M, int piece) { return M <= 4 * piece ? 4 : M <= 512 ? 16 : 64; }
+// Lanes that have a row: the fewest of 4, 8 and 16 that hold it in a piece of 16 bytes each, 16 with two pieces, or 64 and as many as it takes.
+int lanes_of(int M, int piece) { return M <= 4 * piece ? 4 : M <= 8 * piece ? 8 : M <= 32 * piece ? 16 : 64; }
 int pass_blocks(int64_t N, int M, int dtype) {
   if (N == 0) return 0;
-  const int rows = M > kMostInLanes ? 1 : 4 * (64 / lanes_of(M, dtype == FSGS_DTYPE_F32 ? 4 : 8));
+  const int rows = M > kMostInLanes ? 1 : row_threads(M > 2048 ? 64 : 32) / lanes_of(M, dtype == FSGS_DTYPE_F32 ? 4 : 8);
   const int64_t blocks = (N + rows - 1) / rows;
-  return (int) (blocks < kPassBlocks ? blocks : kPassBlocks);
+  return (int) (blocks < kRowBlocks ? blocks : kRowBlocks);
 }
 bool in_lds(int64_t M) { return M <= kMostInLds; }
 int neighbour_blocks(int64_t N) {
@@ -536,29 +676,33 @@ int neighbour_blocks(int64_t N) {
 }
 
 // kernel<T, lanes, values>(...) for the narrowest rows that hold M columns
-#define FSGS_ROW_KERNELS(T, LAUNCH)                      \
-  do {                                                   \
-    constexpr int kPiece = 16 / sizeof(T);               \
-    if (M <= 4 * kPiece) LAUNCH(T, 4, kPiece);           \
-    else if (kPiece == 4 && M <= 64) LAUNCH(T, 16, 4 * (kPiece / 4)); \
-    else if (M <= 128) LAUNCH(T, 16, 8);                 \
-    else if (M <= 256) LAUNCH(T, 16, 16);                \
-    else if (M <= 512) LAUNCH(T, 16, 32);                \
-    else if (M <= 1024) LAUNCH(T, 64, 16);               \
-    else if (M <= 2048) LAUNCH(T, 64, 32);               \
-    else LAUNCH(T, 64, 64);                              \
+#define FSGS_ROW_KERNELS(T, LAUNCH)                         \
+  do {                                                      \
+    constexpr int kPiece = 16 / sizeof(T);                  \
+    if (M <= 4 * kPiece) LAUNCH(T, 4, kPiece);              \
+    else if (M <= 8 * kPiece) LAUNCH(T, 8, kPiece);         \
+    else if (M <= 16 * kPiece) LAUNCH(T, 16, kPiece);       \
+    else if (M <= 32 * kPiece) LAUNCH(T, 16, 2 * kPiece);   \
+    else if (M <= 64 * kPiece) LAUNCH(T, 64, kPiece);       \
+    else if (M <= 512) LAUNCH(T, 64, 8);                    \
+    else if (M <= 1024) LAUNCH(T, 64, 16);                  \
+    else if (M <= 2048) LAUNCH(T, 64, 32);                  \
+    else LAUNCH(T, 64, 64);                                 \
   } while (0)
 
 template <typename T>
 void launch_rows(int G, int64_t N, int M, int64_t ld, int K, const void* logits, const uint8_t* rows, float2* stats, float* sums,
                  int* counts, BlockRows* blocks, unsigned* ticket, hipStream_t s) {
   const T* x = (const T*) logits;
-#define LAUNCH(T, L, V) \
-  hipLaunchKernelGGL((balance_rows_kernel<T, L, V>), dim3(G), dim3(256), 0, s, N, M, ld, K, x, rows, stats, sums, counts, blocks, ticket)
-  if (M > kMostInLanes)
+  if (M > kMostInLanes) {
     hipLaunchKernelGGL((balance_wide_kernel<T>), dim3(G), dim3(256), 0, s, N, M, ld, K, x, rows, stats, sums, counts, blocks, ticket);
-  else
-    FSGS_ROW_KERNELS(T, LAUNCH);
+    return;
+  }
+  const bool whole = M % (16 / sizeof(T)) == 0 && ld * sizeof(T) % 16 == 0 && (uintptr_t) logits % 16 == 0;
+#define LAUNCH(T, L, V)                                                                                                          \
+  hipLaunchKernelGGL((whole ? balance_rows_kernel<T, L, V, true> : balance_rows_kernel<T, L, V, false>), dim3(G), dim3(row_threads(V)), 0, \
+                     s, N, M, ld, K, x, rows, stats, sums, counts, blocks, ticket)
+  FSGS_ROW_KERNELS(T, LAUNCH);
 #undef LAUNCH
 }
 
@@ -567,14 +711,16 @@ void launch_rows_backward(int G, int64_t N, int M, int64_t ld, const void* logit
                           const int64_t* totals, const float* g_loss, const float* g_importance, void* grad, hipStream_t s) {
   const T* x = (const T*) logits;
   T* out = (T*) grad;
-#define LAUNCH(T, L, V)                                                                                                            \
-  hipLaunchKernelGGL((balance_rows_backward_kernel<T, L, V>), dim3(G), dim3(256), 0, s, N, M, ld, x, stats, counts, totals, g_loss, \
-                     g_importance, out)
-  if (M > kMostInLanes)
+  if (M > kMostInLanes) {
     hipLaunchKernelGGL((balance_wide_backward_kernel<T>), dim3(G), dim3(256), 0, s, N, M, ld, x, stats, counts, totals, g_loss,
                        g_importance, out);
-  else
-    FSGS_ROW_KERNELS(T, LAUNCH);
+    return;
+  }
+  const bool whole = M % (16 / sizeof(T)) == 0 && ld * sizeof(T) % 16 == 0 && ((uintptr_t) logits | (uintptr_t) grad) % 16 == 0;
+#define LAUNCH(T, L, V)                                                                                                             \
+  hipLaunchKernelGGL((whole ? balance_rows_backward_kernel<T, L, V, true> : balance_rows_backward_kernel<T, L, V, false>), dim3(G), \
+                     dim3(256), 0, s, N, M, ld, x, stats, counts, totals, g_loss, g_importance, out)
+  FSGS_ROW_KERNELS(T, LAUNCH);
 #undef LAUNCH
 }
 #undef FSGS_ROW_KERNELS
@@ -619,7 +765,7 @@ FSGS_API int fsgs_balance_loss_forward(int64_t N, int M, int64_t ld, int K, int 
     launch(G, N, M, ld, K, logits, rows, (float2*) stats, sums, block_counts, blocks, ticket, s);
   }
   if (const int rc = check_launch(what)) return rc;
-  hipLaunchKernelGGL(balance_totals_kernel<float>, dim3(div_up(M, 32)), dim3(1024), 0, s, G, G, M, sums, block_counts, blocks,
+  hipLaunchKernelGGL(balance_totals_kernel<float>, dim3(div_up(M, kTotalColumns)), dim3(1024), 0, s, G, G, M, sums, block_counts, blocks,
                      (double*) (at + ws.parts), ticket, loss, counts, importance, totals);
   return check_launch(what);
 }
@@ -664,14 +810,15 @@ FSGS_API int fsgs_neighbour_balance_forward(int64_t N, int M, int K, const float
   if (!in_lds(M)) hipLaunchKernelGGL(clear_kernel, dim3(div_up(M, 256)), dim3(256), 0, s, M, sums, block_counts);
   if (G == 0)
     hipLaunchKernelGGL(clear_kernel, dim3(1), dim3(256), 0, s, 1, (unsigned long long*) ticket, (int*) ticket + 2);
-  else if (in_lds(M))
-    hipLaunchKernelGGL(balance_neighbours_kernel<true>, dim3(G), dim3(kNeighbourThreads), (size_t) M * 12, s, N, M, K, weights, indices,
-                       rows, sums, block_counts, blocks, ticket);
-  else
-    hipLaunchKernelGGL(balance_neighbours_kernel<false>, dim3(G), dim3(kNeighbourThreads), 0, s, N, M, K, weights, indices, rows, sums,
+  else {
+    const bool quads = K % 4 == 0 && ((uintptr_t) weights | (uintptr_t) indices) % 16 == 0;
+    auto kernel = in_lds(M) ? (quads ? balance_neighbours_kernel<true, true> : balance_neighbours_kernel<true, false>)
+                            : (quads ? balance_neighbours_kernel<false, true> : balance_neighbours_kernel<false, false>);
+    hipLaunchKernelGGL(kernel, dim3(G), dim3(kNeighbourThreads), in_lds(M) ? (size_t) M * 12 : 0, s, N, M, K, weights, indices, rows, sums,
                        block_counts, blocks, ticket);
+  }
   if (const int rc = check_launch(what)) return rc;
-  hipLaunchKernelGGL(balance_totals_kernel<unsigned long long>, dim3(div_up(M, 32)), dim3(1024), 0, s, G_sums, G, M, sums, block_counts,
+  hipLaunchKernelGGL(balance_totals_kernel<unsigned long long>, dim3(div_up(M, kTotalColumns)), dim3(1024), 0, s, G_sums, G, M, sums, block_counts,
                      blocks, (double*) (at + ws.parts), ticket, loss, counts, importance, totals);
   return check_launch(what);
 }
@@ -683,8 +830,10 @@ FSGS_API int fsgs_neighbour_balance_backward(int64_t N, int M, int K, const int6
   if (N == 0) return kOk;
   FSGS_REQUIRE(indices && counts && totals && grad && (g_loss || g_importance), "%s: null pointer", what);
   FSGS_REQUIRE((uintptr_t) indices % 8 == 0 && (uintptr_t) grad % 4 == 0, "%s: misaligned address", what);
-  const int64_t blocks = (N * K + 255) / 256;
-  hipLaunchKernelGGL(balance_neighbours_backward_kernel, dim3((unsigned) (blocks < 8192 ? blocks : 8192)), dim3(256), 0,
+  const int64_t blocks = (N * K + 4 * kSlopeThreads - 1) / (4 * kSlopeThreads);
+  const bool lds = M <= kMostSlopes;
+  hipLaunchKernelGGL((lds ? balance_neighbours_backward_kernel<true> : balance_neighbours_backward_kernel<false>),
+                     dim3((unsigned) (blocks < kSlopeBlocks ? blocks : kSlopeBlocks)), dim3(kSlopeThreads), lds ? (size_t) M * 4 : 0,
                      (hipStream_t) stream, N, M, K, indices, rows, counts, totals, g_loss, g_importance, grad);
   return check_launch(what);
 }
