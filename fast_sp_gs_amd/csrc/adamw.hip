@@ -83,11 +83,25 @@ __device__ __forceinline__ __half from_float<__half>(float x) { return __float2h
 template <>
 __device__ __forceinline__ __hip_bfloat16 from_float<__hip_bfloat16>(float x) { return __float2bfloat16(x); }
 
+// One access of sizeof(Q) bytes; `kStream`: past the caches, which what is touched once a step would empty.
+template <bool kStream, typename Q>
+__device__ __forceinline__ Q get(const void* p) {
+  typedef uint32_t Raw __attribute__((ext_vector_type(sizeof(Q) / 4)));
+  const Raw raw = kStream ? __builtin_nontemporal_load((const Raw*) p) : *(const Raw*) p;
+  return __builtin_bit_cast(Q, raw);
+}
+template <bool kStream, typename Q>
+__device__ __forceinline__ void put(void* p, const Q& q) {
+  typedef uint32_t Raw __attribute__((ext_vector_type(sizeof(Q) / 4)));
+  if (kStream) __builtin_nontemporal_store(__builtin_bit_cast(Raw, q), (Raw*) p);
+  else *(Raw*) p = __builtin_bit_cast(Raw, q);
+}
+
 // `left` elements are there; `whole`: all four, and their address allows one access.
-template <typename T>
+template <bool kStream, typename T>
 __device__ __forceinline__ void load4(const T* p, int64_t left, bool whole, float out[4]) {
   if (whole) {
-    const Four<T> q = *(const Four<T>*) p;
+    const Four<T> q = get<kStream, Four<T>>(p);
 #pragma unroll
     for (int k = 0; k < 4; ++k) out[k] = to_float(q.x[k]);
   } else {
@@ -95,13 +109,13 @@ __device__ __forceinline__ void load4(const T* p, int64_t left, bool whole, floa
     for (int k = 0; k < 4; ++k) out[k] = k < left ? to_float(p[k]) : 0.0f;
   }
 }
-template <typename T>
+template <bool kStream, typename T>
 __device__ __forceinline__ void store4(T* p, int64_t left, bool whole, const float in[4]) {
   if (whole) {
     Four<T> q;
 #pragma unroll
     for (int k = 0; k < 4; ++k) q.x[k] = from_float<T>(in[k]);
-    *(Four<T>*) p = q;
+    put<kStream>(p, q);
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -124,7 +138,7 @@ __device__ __forceinline__ float updated(const Step& s, const Rates& r, float ke
 }
 
 // ---- 32-bit moments -------------------------------------------------------------------------------------------------------------
-template <typename T>
+template <typename T, bool kStream>
 __global__ void __launch_bounds__(256) adamw_kernel(AdamwTable t, Step s, const float* __restrict__ factor,
                                                     const Rates* __restrict__ rates) {
   const int q = tensor_of(t.first_block, t.n, blockIdx.x);
@@ -138,12 +152,12 @@ __global__ void __launch_bounds__(256) adamw_kernel(AdamwTable t, Step s, const 
   const bool whole = left >= 4 && (((uintptr_t) first | (uintptr_t) second) & 15) == 0 &&
                      (((uintptr_t) param | (uintptr_t) grad) & (4 * sizeof(T) - 1)) == 0;
   float p[4], g[4], m[4], v[4];
-  load4(param, left, whole, p), load4(grad, left, whole, g);
-  load4<float>(first, left, whole, m), load4<float>(second, left, whole, v);
+  load4<kStream>(param, left, whole, p), load4<kStream>(grad, left, whole, g);
+  load4<kStream>(first, left, whole, m), load4<kStream>(second, left, whole, v);
 #pragma unroll
   for (int k = 0; k < 4; ++k) p[k] = updated(s, r, keep, eps, p[k], c * g[k], m[k], v[k]);
-  store4(param, left, whole, p);
-  store4<float>(first, left, whole, m), store4<float>(second, left, whole, v);
+  store4<kStream>(param, left, whole, p);
+  store4<kStream>(first, left, whole, m), store4<kStream>(second, left, whole, v);
 }
 
 // ---- 8-bit moments ----------------------------------------------------------------------------------------------------------------
@@ -234,7 +248,7 @@ __host__ __device__ __forceinline__ StateView view_state(void* state, int64_t co
 }
 
 // A wavefront steps a block: a lane has four elements of it.
-template <typename T>
+template <typename T, bool kStream>
 __global__ void __launch_bounds__(256) adamw8_kernel(AdamwTable t, Step s, const float* __restrict__ factor,
                                                      const Rates* __restrict__ rates) {
   const int q = tensor_of(t.first_block, t.n, blockIdx.x);
@@ -249,8 +263,8 @@ __global__ void __launch_bounds__(256) adamw8_kernel(AdamwTable t, Step s, const
   const StateView state = view_state(t.m[q], t.count[q]);
   const bool whole = left >= 4 && (((uintptr_t) param | (uintptr_t) grad) & (4 * sizeof(T) - 1)) == 0;
   float p[4], g[4], m[4], v[4];
-  load4(param, left, whole, p), load4(grad, left, whole, g);
-  const uint32_t old_m = *(const uint32_t*) (state.m + e), old_v = *(const uint32_t*) (state.v + e);
+  load4<kStream>(param, left, whole, p), load4<kStream>(grad, left, whole, g);
+  const uint32_t old_m = get<kStream, uint32_t>(state.m + e), old_v = get<kStream, uint32_t>(state.v + e);
   int exponent_m = state.exponents[2 * block], exponent_v = state.exponents[2 * block + 1];
   decode4(old_m, old_v, exponent_m, exponent_v, m, v);
   uint32_t noise[4];
@@ -262,8 +276,8 @@ __global__ void __launch_bounds__(256) adamw8_kernel(AdamwTable t, Step s, const
   }
   uint32_t codes_m, codes_v;
   encode4(m, v, noise, codes_m, codes_v, exponent_m, exponent_v);
-  store4(param, left, whole, p);
-  *(uint32_t*) (state.m + e) = codes_m, *(uint32_t*) (state.v + e) = codes_v;
+  store4<kStream>(param, left, whole, p);
+  put<kStream>(state.m + e, codes_m), put<kStream>(state.v + e, codes_v);
   if (lane == 0) *(uint16_t*) (state.exponents + 2 * block) = (uint16_t) (exponent_m | exponent_v << 8);
 }
 
@@ -277,7 +291,7 @@ struct MomentsTable {
 };
 
 // The values that 8-bit moments stand for; a lane writes 16 bytes of each.
-template <typename T>
+template <typename T, bool kStream>
 __global__ void __launch_bounds__(256) adamw8_unpack_kernel(MomentsTable t) {
   constexpr int kWords = 4 / sizeof(T);  // of four codes
   const int q = tensor_of(t.first_block, t.n, blockIdx.x);
@@ -287,16 +301,18 @@ __global__ void __launch_bounds__(256) adamw8_unpack_kernel(MomentsTable t) {
   T *first = (T*) t.m[q] + e, *second = (T*) t.v[q] + e;
   const int exponent_m = state.exponents[2 * (e / kBlock)], exponent_v = state.exponents[2 * (e / kBlock) + 1];
   const bool whole = left >= 4 * kWords && (((uintptr_t) first | (uintptr_t) second) & 15) == 0;
-  struct alignas(16) { T x[4 * kWords]; } pm, pv;
+  struct alignas(16) Values { T x[4 * kWords]; } pm, pv;
+  struct alignas(4 * kWords) Codes { uint32_t x[kWords]; };
+  const Codes codes_m = get<kStream, Codes>(state.m + e), codes_v = get<kStream, Codes>(state.v + e);
 #pragma unroll
   for (int w = 0; w < kWords; ++w) {
     float m[4], v[4];
-    decode4(*(const uint32_t*) (state.m + e + 4 * w), *(const uint32_t*) (state.v + e + 4 * w), exponent_m, exponent_v, m, v);
+    decode4(codes_m.x[w], codes_v.x[w], exponent_m, exponent_v, m, v);
 #pragma unroll
     for (int k = 0; k < 4; ++k) pm.x[4 * w + k] = from_float<T>(m[k]), pv.x[4 * w + k] = from_float<T>(v[k]);
   }
   if (whole) {
-    *(decltype(pm)*) first = pm, *(decltype(pv)*) second = pv;
+    put<kStream>(first, pm), put<kStream>(second, pv);
   } else {
 #pragma unroll
     for (int k = 0; k < 4 * kWords; ++k)
@@ -313,7 +329,7 @@ __global__ void __launch_bounds__(256) adamw8_pack_kernel(MomentsTable t) {
   const int64_t e = block * kBlock + lane * 4, left = t.count[q] - e;
   const StateView state = view_state(t.state[q], t.count[q]);
   float m[4], v[4];
-  load4((const float*) t.m[q] + e, left, false, m), load4((const float*) t.v[q] + e, left, false, v);
+  load4<false>((const float*) t.m[q] + e, left, false, m), load4<false>((const float*) t.v[q] + e, left, false, v);
   const uint32_t noise[4] = {0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
   uint32_t codes_m, codes_v;
   int exponent_m, exponent_v;
@@ -340,7 +356,7 @@ __device__ __forceinline__ double block_sum(double x, double* s_wave) {
 }
 
 // Sums of squares: a lane's 32 elements of a chunk in float32 (four sums of eight), everything above in float64.
-template <typename T>
+template <typename T, bool kStream>
 __global__ void __launch_bounds__(256) square_sums_kernel(NormTable t, double* __restrict__ sums) {
   __shared__ double s_wave[4];
   double total = 0.0;
@@ -355,7 +371,7 @@ __global__ void __launch_bounds__(256) square_sums_kernel(NormTable t, double* _
       const int64_t e = at + j * 1024;
       if (e >= count) break;
       float g[4];
-      load4(grad + e, count - e, aligned && count - e >= 4, g);
+      load4<kStream>(grad + e, count - e, aligned && count - e >= 4, g);
 #pragma unroll
       for (int k = 0; k < 4; ++k) sum[k] = fmaf(g[k], g[k], sum[k]);
     }
@@ -400,6 +416,22 @@ enum Type { kFloat32 = FSGS_DTYPE_F32, kFloat16 = FSGS_DTYPE_F16, kBfloat16 = FS
 size_t type_size(int type) { return type == kFloat32 ? 4 : 2; }
 bool is_type(int type) { return type == kFloat32 || type == kFloat16 || type == kBfloat16; }
 
+// A launch that moves this many bytes goes past the caches: less may still be, or stay, in the 256 MB memory-side cache. us of a step of n
+// elements, three sets of tensors in turn, ordinary and streaming accesses: float32 4M (117 MB) 19.4 and 23.0, 8M 47.2 and 43.6, 16M
+// 91.3 and 84.4, 64M 345 and 324; bfloat16 4M 16.5 and 17.4, 8M (185 MB) 35.3 and 33.4, 64M 267 and 245; 8-bit moments, float32 8M
+// (134 MB) 27.1 and 29.3, 16M 57.1 and 53.1, 64M 198 and 186; read back in bfloat16 16M (101 MB) 17.7 and 20.7, 64M 72.7 and 67.9.
+bool streams(int n, const int64_t* count, size_t bytes_an_element) {
+  constexpr int64_t kStreamBytes = (int64_t) 160 << 20;
+  int64_t sum = 0;
+  for (int q = 0; q < n; ++q) sum += count[q];
+  return sum >= kStreamBytes / (int64_t) bytes_an_element;
+}
+// kernel<type, streaming>
+#define FSGS_BY_TYPE(kernel, dtype, stream)                                                          \
+  ((dtype) == kFloat32   ? ((stream) ? kernel<float, true> : kernel<float, false>)                   \
+   : (dtype) == kFloat16 ? ((stream) ? kernel<__half, true> : kernel<__half, false>)                 \
+                         : ((stream) ? kernel<__hip_bfloat16, true> : kernel<__hip_bfloat16, false>))
+
 // first[q]: blocks before tensor q at `per_block` elements a block
 template <typename Table>
 int lay_out(const char* what, Table& t, unsigned* first, int n, const int64_t* count, int64_t per_block) {
@@ -439,7 +471,7 @@ FSGS_API int fsgs_grad_square_sums(int n_tensors, int dtype, const int64_t* coun
     FSGS_REQUIRE(count[q] == 0 || (grad[q] && (uintptr_t) grad[q] % type_size(dtype) == 0), "%s: bad tensor %d", what, q);
     t.grad[q] = grad[q];
   }
-  auto kernel = dtype == kFloat32 ? square_sums_kernel<float> : dtype == kFloat16 ? square_sums_kernel<__half> : square_sums_kernel<__hip_bfloat16>;
+  auto kernel = FSGS_BY_TYPE(square_sums_kernel, dtype, streams(n_tensors, count, type_size(dtype)));
   hipLaunchKernelGGL(kernel, dim3(n_sums), dim3(256), 0, (hipStream_t) stream, t, sums);
   return check_launch(what);
 }
@@ -478,7 +510,7 @@ int adamw_update(const char* what, int bits, int n, int dtype, const int64_t* co
   if (t.first_block[n] == 0) return kOk;
   for (int q = 0; q < n; ++q) {
     const uintptr_t wide = (uintptr_t) m[q] | (v ? (uintptr_t) v[q] : 0), narrow = (uintptr_t) param[q] | (uintptr_t) grad[q];
-    FSGS_REQUIRE(count[q] == 0 || (param[q] && grad[q] && m[q] && (!v || v[q]) && wide % 4 == 0 && narrow % type_size(dtype) == 0),
+    FSGS_REQUIRE(count[q] == 0 || (param[q] && grad[q] && m[q] && (!v || v[q]) && wide % (bits == 8 ? 16 : 4) == 0 && narrow % type_size(dtype) == 0),
                  "%s: bad tensor %d", what, q);
     t.param[q] = param[q], t.grad[q] = grad[q], t.m[q] = m[q], t.v[q] = v ? v[q] : nullptr;
     t.keep[q] = (float) (1.0 - lr[q] * decay[q]), t.eps[q] = (float) eps[q];
@@ -489,8 +521,8 @@ int adamw_update(const char* what, int bits, int n, int dtype, const int64_t* co
     t.rates[q].key         = noise_key((uint32_t) (int64_t) step[q], seed);
   }
   const Step s{(float) b1, (float) b2, (float) (1.0 - b1), (float) (1.0 - b2)};
-  auto kernel = bits == 8 ? (dtype == kFloat32 ? adamw8_kernel<float> : dtype == kFloat16 ? adamw8_kernel<__half> : adamw8_kernel<__hip_bfloat16>)
-                          : (dtype == kFloat32 ? adamw_kernel<float> : dtype == kFloat16 ? adamw_kernel<__half> : adamw_kernel<__hip_bfloat16>);
+  const bool past = streams(n, count, 3 * type_size(dtype) + (bits == 8 ? 4 : 16));
+  auto kernel = bits == 8 ? FSGS_BY_TYPE(adamw8_kernel, dtype, past) : FSGS_BY_TYPE(adamw_kernel, dtype, past);
   hipLaunchKernelGGL(kernel, dim3(t.first_block[n]), dim3(256), 0, (hipStream_t) stream, t, s, factor, (const Rates*) rates);
   return check_launch(what);
 }
@@ -502,7 +534,7 @@ int moments(const char* what, int n, const int64_t* count, const void* const* st
   FSGS_REQUIRE(count && state && m && v, "%s: null pointer", what);
   if (const int rc = lay_out(what, t, t.first_block, n, count, per_block)) return rc;
   for (int q = 0; q < n; ++q) {
-    FSGS_REQUIRE(count[q] == 0 || (state[q] && m[q] && v[q] && (uintptr_t) state[q] % 4 == 0 &&
+    FSGS_REQUIRE(count[q] == 0 || (state[q] && m[q] && v[q] && (uintptr_t) state[q] % 16 == 0 &&
                                    ((uintptr_t) m[q] | (uintptr_t) v[q]) % size == 0), "%s: bad tensor %d", what, q);
     t.state[q] = (void*) state[q], t.m[q] = (void*) m[q], t.v[q] = (void*) v[q];
   }
@@ -532,7 +564,7 @@ FSGS_API int fsgs_adamw8_unpack_multi(int n_tensors, int dtype, const int64_t* c
   MomentsTable t{};
   if (const int rc = moments(what, n_tensors, count, state, m, v, type_size(dtype), 4096 / type_size(dtype), t)) return rc;
   if (t.first_block[t.n] == 0) return kOk;
-  auto kernel = dtype == kFloat32 ? adamw8_unpack_kernel<float> : dtype == kFloat16 ? adamw8_unpack_kernel<__half> : adamw8_unpack_kernel<__hip_bfloat16>;
+  auto kernel = FSGS_BY_TYPE(adamw8_unpack_kernel, dtype, streams(n_tensors, count, 2 + 2 * type_size(dtype)));
   hipLaunchKernelGGL(kernel, dim3(t.first_block[t.n]), dim3(256), 0, (hipStream_t) stream, t);
   return check_launch(what);
 }

@@ -23,9 +23,10 @@ namespace fsgs {
 namespace {
 
 constexpr int kMostChoices   = 64;
-constexpr int kRowBlocks     = 512;   // of the pass over logits
-// threads of its blocks: with 64 values in each lane a wavefront has the registers of a SIMD to itself
-constexpr int row_threads(int vals) { return vals == 64 ? 256 : 512; }
+constexpr int kRowBlocks     = 768;   // of the pass over logits
+// Threads of its blocks, and wavefronts that share a SIMD's registers: with 64 values in each lane one has them to itself.
+constexpr int row_threads(int vals) { return vals >= 32 ? 256 : 512; }
+constexpr int row_waves(int vals, bool narrow) { return vals == 64 ? 1 : vals == 32 ? (narrow ? 3 : 2) : vals == 16 ? 3 : 4; }
 constexpr int kMostInLanes   = 4096;  // superpoints whose row is held by the lanes of one wavefront
 constexpr int kNeighbourBlocks = 256;
 constexpr int kNeighbourThreads = 1024;
@@ -120,13 +121,21 @@ struct Row {
     }
   }
   // -inf for what there is not; `full`: every lane has kVals columns
+  template <bool kWhole>
   __device__ __forceinline__ void values(float x[kVals], int M, bool full, bool on, int lane) const {
 #pragma unroll
     for (int j = 0; j < kVals; ++j) x[j] = to_float(piece[j / kPiece].x[j % kPiece]);
-    if (wave_ballot(!on) || !full) {
-      const int there = on ? M : 0, l = keep_local(lane);
+    if (wave_ballot(!on)) {
 #pragma unroll
-      for (int j = 0; j < kVals; ++j) x[j] = column<T, kLanes>(l, j) < there ? x[j] : -INFINITY;
+      for (int j = 0; j < kVals; ++j) x[j] = on ? x[j] : -INFINITY;
+    }
+    if (full) return;
+    const int l = keep_local(lane);
+#pragma unroll
+    for (int i = 0; i < kVals; i += kPiece) {
+      if ((i / kPiece + 1) * kLanes * kPiece <= M) continue;  // of all lanes
+#pragma unroll
+      for (int k = 0; k < kPiece; ++k) x[i + k] = column<T, kLanes>(l, i + (kWhole ? 0 : k)) < M ? x[i + k] : -INFINITY;
     }
   }
 };
@@ -143,8 +152,9 @@ __device__ __forceinline__ int reaching(const float x[kVals], float t) {
 // Counts the row's K largest values above -inf, the lowest column first among equals. `lane_top`: the largest of the lane, `top` of the row,
 // ordered. The K-th largest of the lanes' own largest is reached by at least K values, and mostly by no other: 4 of 512 values lie
 // in 4 of 64 lanes in 9 rows of 10. Otherwise the threshold rises value by value, after a walk down from the top where that is nearer.
+// What is chosen among values equal to the threshold is counted in LDS.
 template <typename T, int kLanes, int kVals>
-__device__ __forceinline__ void choose(const float x[kVals], int lane_top, int top, int K, int lane, int count[kVals]) {
+__device__ __forceinline__ void choose(const float x[kVals], int lane_top, int top, int K, int lane, int count[kVals], int* s_count) {
   const int lowest = ordered(-INFINITY);
   int t_ordered = top;
   for (int r = 1; r < K; ++r) t_ordered = row_max<kLanes>(lane_top < t_ordered ? lane_top : lowest);
@@ -163,48 +173,41 @@ __device__ __forceinline__ void choose(const float x[kVals], int lane_top, int t
       const int m = reaching<kLanes, kVals>(x, s);
       if (n > 2 * K) t = s, n = m;
     }
-    for (;;) {
+    bool ties = false;  // more than K reach t, fewer than K what is above it
+    int left = 0;       // of those equal to t
+    float all_from = t;
+    while (wave_ballot(n > K && !ties)) {
       float above = INFINITY;
 #pragma unroll
       for (int j = 0; j < kVals; ++j) above = fminf(above, x[j] > t ? x[j] : INFINITY);
       above = unordered(row_min<kLanes>(ordered(above)));
-      const int m = reaching<kLanes, kVals>(x, above);
-      const bool better = n > K && m >= K && above > t;
-      if (better) t = above, n = m;
-      if (!wave_ballot(better)) break;
+      const int m = above > t ? reaching<kLanes, kVals>(x, above) : 0;
+      if (n > K && !ties) {
+        if (m >= K) t = all_from = above, n = m;
+        else ties = true, left = K - m, all_from = m > 0 ? above : __builtin_nanf("");  // nothing reaches a NaN
+      }
     }
-    const bool ties = n > K;  // of values equal to t
-    if (wave_ballot(ties)) {
-      int greater = 0;
+    int at = -1;
+    while (wave_ballot(left > 0)) {
+      const int l = keep_local(lane);  // or every column's index stays in a register of its own
+      int where = 0x7fffffff;
 #pragma unroll
       for (int j = 0; j < kVals; ++j) {
-        greater += x[j] > t ? 1 : 0;
-        count[j] += (ties ? x[j] > t : x[j] >= t) ? 1 : 0;
+        const int c = column<T, kLanes>(l, j);
+        where = min(where, x[j] == t && c > at ? c : 0x7fffffff);
       }
-      greater = row_count<kLanes>(greater);
-      int left = ties ? K - greater : 0, at = -1;
-      while (wave_ballot(left > 0)) {
-        const int l = keep_local(lane);  // or every column's index stays in a register of its own
-        int where = 0x7fffffff;
-#pragma unroll
-        for (int j = 0; j < kVals; ++j) {
-          const int c = column<T, kLanes>(l, j);
-          where = min(where, x[j] == t && c > at ? c : 0x7fffffff);
-        }
-        at = row_min<kLanes>(where);
-#pragma unroll
-        for (int j = 0; j < kVals; ++j) count[j] += left > 0 && column<T, kLanes>(l, j) == at ? 1 : 0;
-        --left;
-      }
-      return;
+      at = row_min<kLanes>(where);
+      if (left > 0 && lane == 0) atomicAdd(&s_count[at], 1);
+      --left;
     }
+    t = ties ? all_from : t;
   }
 #pragma unroll
   for (int j = 0; j < kVals; ++j) count[j] += x[j] >= t ? 1 : 0;
 }
 
 template <typename T, int kLanes, int kVals, bool kWhole>
-__global__ void __launch_bounds__(row_threads(kVals)) balance_rows_kernel(int64_t N, int M, int64_t ld, int K,
+__global__ void __launch_bounds__(row_threads(kVals), row_waves(kVals, sizeof(T) == 2 && kWhole)) balance_rows_kernel(int64_t N, int M, int64_t ld, int K,
     const T* __restrict__ logits, const uint8_t* __restrict__ rows, float2* __restrict__ stats, float* __restrict__ sums,
     int* __restrict__ counts, BlockRows* __restrict__ blocks, unsigned* __restrict__ ticket) {
   constexpr int kRows = 64 / kLanes, kThreads = row_threads(kVals), kWaves = kThreads / 64;
@@ -218,6 +221,8 @@ __global__ void __launch_bounds__(row_threads(kVals)) balance_rows_kernel(int64_
   int count[kVals], counted = 0;
 #pragma unroll
   for (int j = 0; j < kVals; ++j) sum[j] = 0.0f, count[j] = 0;
+  for (int c = threadIdx.x; c < kLanes * kVals; c += kThreads) s_count[c] = 0;
+  __syncthreads();
   const int64_t step = (int64_t) gridDim.x * kWaves * kRows;
   int64_t base = ((int64_t) blockIdx.x * kWaves + wave) * kRows;
 
@@ -227,12 +232,12 @@ __global__ void __launch_bounds__(row_threads(kVals)) balance_rows_kernel(int64_
   auto address = [&](int64_t row, bool on) { return logits + (on ? row : 0) * ld; };
   auto work = [&](const Row<T, kLanes, kVals>& row, int64_t at, bool on) {
     float x[kVals];
-    row.values(x, M, full, on, lane);
+    row.template values<kWhole>(x, M, full, on, lane);
     float lane_top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < kVals; ++j) lane_top = fmaxf(lane_top, x[j]);
     const int lane_top_ordered = ordered(lane_top), top_ordered = row_max<kLanes>(lane_top_ordered);
-    choose<T, kLanes, kVals>(x, lane_top_ordered, top_ordered, K, lane, count);
+    choose<T, kLanes, kVals>(x, lane_top_ordered, top_ordered, K, lane, count, s_count);
     // a row without a number (top is -inf): the sum is 0, or NaN where one of its values is, which counts
     const float top = unordered(top_ordered), shift = top == -INFINITY ? 0.0f : top;
     float total = 0.0f;
@@ -271,12 +276,13 @@ __global__ void __launch_bounds__(row_threads(kVals)) balance_rows_kernel(int64_
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) counted += __shfl_xor(counted, d);
   if ((threadIdx.x & 63) == 0) s_rows[wave] = counted;
+  __syncthreads();  // ties are counted
   for (int w = 0; w < kWaves; ++w) {
     if (w == wave && group == 0)
 #pragma unroll
       for (int j = 0; j < kVals; ++j) {
         const int c = column<T, kLanes>(lane, j);
-        s_sum[c] = w ? s_sum[c] + sum[j] : sum[j], s_count[c] = w ? s_count[c] + count[j] : count[j];
+        s_sum[c] = w ? s_sum[c] + sum[j] : sum[j], s_count[c] += count[j];
       }
     __syncthreads();
   }
@@ -317,7 +323,7 @@ __global__ void __launch_bounds__(256) balance_rows_backward_kernel(int64_t N, i
   auto work = [&](const Row<T, kLanes, kVals>& row, int64_t at, float2 stat) {
     const bool on = on_of(at, stat);
     float x[kVals], mean = 0.0f;
-    row.values(x, M, full, on, lane);
+    row.template values<kWhole>(x, M, full, on, lane);
 #pragma unroll
     for (int j = 0; j < kVals; ++j) {
       x[j] = __builtin_amdgcn_exp2f((x[j] - stat.x) * kLog2e) * stat.y;
@@ -665,7 +671,7 @@ struct Workspace {
 int lanes_of(int M, int piece) { return M <= 4 * piece ? 4 : M <= 8 * piece ? 8 : M <= 32 * piece ? 16 : 64; }
 int pass_blocks(int64_t N, int M, int dtype) {
   if (N == 0) return 0;
-  const int rows = M > kMostInLanes ? 1 : row_threads(M > 2048 ? 64 : 32) / lanes_of(M, dtype == FSGS_DTYPE_F32 ? 4 : 8);
+  const int rows = M > kMostInLanes ? 1 : row_threads(M > 1024 ? 32 : 16) / lanes_of(M, dtype == FSGS_DTYPE_F32 ? 4 : 8);
   const int64_t blocks = (N + rows - 1) / rows;
   return (int) (blocks < kRowBlocks ? blocks : kRowBlocks);
 }
@@ -778,7 +784,8 @@ FSGS_API int fsgs_balance_loss_backward(int64_t N, int M, int64_t ld, int dtype,
   FSGS_REQUIRE(logits && stats && counts && totals && grad && (g_loss || g_importance), "%s: null pointer", what);
   const size_t size = dtype == FSGS_DTYPE_F32 ? 4 : 2;
   FSGS_REQUIRE(((uintptr_t) logits | (uintptr_t) grad) % size == 0 && (uintptr_t) stats % 8 == 0, "%s: misaligned address", what);
-  const int rows = M > kMostInLanes ? 1 : 4 * (64 / lanes_of(M, (int) (16 / size)));
+  // four rows in turn at least for a wavefront, which has its columns' slopes to form first
+  const int rows = M > kMostInLanes ? 1 : 16 * (64 / lanes_of(M, (int) (16 / size)));
   const int64_t blocks = (N + rows - 1) / rows;
   const int G = (int) (blocks < 4096 ? blocks : 4096);
   auto launch = dtype == FSGS_DTYPE_F32 ? launch_rows_backward<float> : dtype == FSGS_DTYPE_F16 ? launch_rows_backward<__half> : launch_rows_backward<__hip_bfloat16>;
