@@ -97,29 +97,29 @@ __device__ __forceinline__ void put(void* p, const Q& q) {
   else *(Raw*) p = __builtin_bit_cast(Raw, q);
 }
 
-// `left` elements are there; `whole`: all four, and their address allows one access.
-template <bool kStream, typename T>
-__device__ __forceinline__ void load4(const T* p, int64_t left, bool whole, float out[4]) {
-  if (whole) {
-    const Four<T> q = get<kStream, Four<T>>(p);
+// Four elements as they lie in memory. `kWhole`: all are there, and their address allows one access; otherwise `left` of them are. Loads of
+// a whole block stand one behind the other, with no branch and no conversion between them: a wavefront waits for memory once.
+template <bool kWhole, bool kStream, typename T>
+__device__ __forceinline__ Four<T> load4(const T* p, int64_t left) {
+  if (kWhole) return get<kStream, Four<T>>(p);
+  Four<T> q;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) out[k] = to_float(q.x[k]);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) out[k] = k < left ? to_float(p[k]) : 0.0f;
-  }
+  for (int k = 0; k < 4; ++k)
+    if (k < left) q.x[k] = p[k];
+    else q.x[k] = from_float<T>(0.0f);
+  return q;
 }
-template <bool kStream, typename T>
-__device__ __forceinline__ void store4(T* p, int64_t left, bool whole, const float in[4]) {
-  if (whole) {
-    Four<T> q;
+template <bool kWhole, bool kStream, typename T>
+__device__ __forceinline__ void store4(T* p, int64_t left, const float in[4]) {
+  Four<T> q;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) q.x[k] = from_float<T>(in[k]);
+  for (int k = 0; k < 4; ++k) q.x[k] = from_float<T>(in[k]);
+  if (kWhole) {
     put<kStream>(p, q);
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (k < left) p[k] = from_float<T>(in[k]);
+      if (k < left) p[k] = q.x[k];
   }
 }
 
@@ -138,26 +138,55 @@ __device__ __forceinline__ float updated(const Step& s, const Rates& r, float ke
 }
 
 // ---- 32-bit moments -------------------------------------------------------------------------------------------------------------
+// What a block needs of its tensor, in scalar registers.
+template <typename T>
+struct Part {
+  T* param;
+  const T* grad;
+  void* m;
+  float* v;
+  int64_t count, first;  // first: of the block's elements
+  Rates rate;
+  float clip, keep, eps;
+  bool aligned;  // param and grad, for four elements at once
+
+  __device__ __forceinline__ Part(const AdamwTable& t, const float* factor, const Rates* rates) {
+    const int q = tensor_of(t.first_block, t.n, blockIdx.x);
+    param = (T*) t.param[q], grad = (const T*) t.grad[q], m = t.m[q], v = t.v[q], count = t.count[q];
+    first = (int64_t) (blockIdx.x - t.first_block[q]) * 1024;
+    rate = t.rates[q], keep = t.keep[q], eps = t.eps[q], clip = 1.0f;
+    if (rates) {
+      const Rates on_device = rates[q];
+      rate = on_device;
+    }
+    if (factor) clip = factor[1];
+    aligned = (((uintptr_t) param | (uintptr_t) grad) & (4 * sizeof(T) - 1)) == 0;
+  }
+};
+
+template <typename T, bool kStream, bool kWhole>
+__device__ __forceinline__ void adamw_block(const Part<T>& t, const Step& s) {
+  const int64_t e = t.first + threadIdx.x * 4, left = t.count - e;
+  if (!kWhole && left <= 0) return;
+  float *first = (float*) t.m + e, *second = t.v + e;
+  const Four<T> param = load4<kWhole, kStream>(t.param + e, left), grad = load4<kWhole, kStream>(t.grad + e, left);
+  Four<float> m = load4<kWhole, kStream>(first, left), v = load4<kWhole, kStream>(second, left);
+  float p[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    p[k] = updated(s, t.rate, t.keep, t.eps, to_float(param.x[k]), t.clip * to_float(grad.x[k]), m.x[k], v.x[k]);
+  store4<kWhole, kStream>(t.param + e, left, p);
+  store4<kWhole, kStream>(first, left, m.x), store4<kWhole, kStream>(second, left, v.x);
+}
+
 template <typename T, bool kStream>
 __global__ void __launch_bounds__(256) adamw_kernel(AdamwTable t, Step s, const float* __restrict__ factor,
                                                     const Rates* __restrict__ rates) {
-  const int q = tensor_of(t.first_block, t.n, blockIdx.x);
-  const int64_t e = (int64_t) (blockIdx.x - t.first_block[q]) * 1024 + threadIdx.x * 4, left = t.count[q] - e;
-  if (left <= 0) return;
-  const Rates r = rates ? rates[q] : t.rates[q];
-  const float c = factor ? factor[1] : 1.0f, keep = t.keep[q], eps = t.eps[q];
-  T* param = (T*) t.param[q] + e;
-  const T* grad = (const T*) t.grad[q] + e;
-  float *first = (float*) t.m[q] + e, *second = t.v[q] + e;
-  const bool whole = left >= 4 && (((uintptr_t) first | (uintptr_t) second) & 15) == 0 &&
-                     (((uintptr_t) param | (uintptr_t) grad) & (4 * sizeof(T) - 1)) == 0;
-  float p[4], g[4], m[4], v[4];
-  load4<kStream>(param, left, whole, p), load4<kStream>(grad, left, whole, g);
-  load4<kStream>(first, left, whole, m), load4<kStream>(second, left, whole, v);
-#pragma unroll
-  for (int k = 0; k < 4; ++k) p[k] = updated(s, r, keep, eps, p[k], c * g[k], m[k], v[k]);
-  store4<kStream>(param, left, whole, p);
-  store4<kStream>(first, left, whole, m), store4<kStream>(second, left, whole, v);
+  const Part<T> part(t, factor, rates);
+  if (part.aligned && (((uintptr_t) part.m | (uintptr_t) part.v) & 15) == 0 && part.first + 1024 <= part.count)
+    adamw_block<T, kStream, true>(part, s);
+  else
+    adamw_block<T, kStream, false>(part, s);
 }
 
 // ---- 8-bit moments ----------------------------------------------------------------------------------------------------------------
@@ -248,37 +277,38 @@ __host__ __device__ __forceinline__ StateView view_state(void* state, int64_t co
 }
 
 // A wavefront steps a block: a lane has four elements of it.
+template <typename T, bool kStream, bool kWhole>
+__device__ __forceinline__ void adamw8_block(const Part<T>& t, const Step& s, int64_t block) {
+  const int lane = threadIdx.x & 63;
+  const int64_t e = block * kBlock + lane * 4, left = t.count - e;
+  const StateView state = view_state(t.m, t.count);
+  const Four<T> param = load4<kWhole, kStream>(t.param + e, left), grad = load4<kWhole, kStream>(t.grad + e, left);
+  uint32_t codes_m = get<kStream, uint32_t>(state.m + e), codes_v = get<kStream, uint32_t>(state.v + e);
+  const int exponents = __builtin_amdgcn_readfirstlane(*(const uint16_t*) (state.exponents + 2 * block));
+  float m[4], v[4], p[4];
+  uint32_t noise[4];
+  decode4(codes_m, codes_v, exponents & 255, exponents >> 8, m, v);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    p[k] = updated(s, t.rate, t.keep, t.eps, to_float(param.x[k]), t.clip * to_float(grad.x[k]), m[k], v[k]);
+    if (!kWhole && k >= left) m[k] = v[k] = 0.0f;
+    noise[k] = mixed((uint32_t) (e + k) * kStride + t.rate.key);
+  }
+  int exponent_m, exponent_v;
+  encode4(m, v, noise, codes_m, codes_v, exponent_m, exponent_v);
+  store4<kWhole, kStream>(t.param + e, left, p);
+  put<kStream>(state.m + e, codes_m), put<kStream>(state.v + e, codes_v);
+  if (lane == 0) *(uint16_t*) (state.exponents + 2 * block) = (uint16_t) (exponent_m | exponent_v << 8);
+}
+
 template <typename T, bool kStream>
 __global__ void __launch_bounds__(256) adamw8_kernel(AdamwTable t, Step s, const float* __restrict__ factor,
                                                      const Rates* __restrict__ rates) {
-  const int q = tensor_of(t.first_block, t.n, blockIdx.x);
-  const int64_t block = (int64_t) (blockIdx.x - t.first_block[q]) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (block * kBlock >= t.count[q]) return;  // the whole wavefront
-  const int64_t e = block * kBlock + lane * 4, left = t.count[q] - e;
-  const Rates rate = rates ? rates[q] : t.rates[q];
-  const float c = factor ? factor[1] : 1.0f, keep = t.keep[q], eps = t.eps[q];
-  T* param = (T*) t.param[q] + e;
-  const T* grad = (const T*) t.grad[q] + e;
-  const StateView state = view_state(t.m[q], t.count[q]);
-  const bool whole = left >= 4 && (((uintptr_t) param | (uintptr_t) grad) & (4 * sizeof(T) - 1)) == 0;
-  float p[4], g[4], m[4], v[4];
-  load4<kStream>(param, left, whole, p), load4<kStream>(grad, left, whole, g);
-  const uint32_t old_m = get<kStream, uint32_t>(state.m + e), old_v = get<kStream, uint32_t>(state.v + e);
-  int exponent_m = state.exponents[2 * block], exponent_v = state.exponents[2 * block + 1];
-  decode4(old_m, old_v, exponent_m, exponent_v, m, v);
-  uint32_t noise[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    p[k] = updated(s, rate, keep, eps, p[k], c * g[k], m[k], v[k]);
-    if (k >= left) m[k] = v[k] = 0.0f;
-    noise[k] = mixed((uint32_t) (e + k) * kStride + rate.key);
-  }
-  uint32_t codes_m, codes_v;
-  encode4(m, v, noise, codes_m, codes_v, exponent_m, exponent_v);
-  store4<kStream>(param, left, whole, p);
-  put<kStream>(state.m + e, codes_m), put<kStream>(state.v + e, codes_v);
-  if (lane == 0) *(uint16_t*) (state.exponents + 2 * block) = (uint16_t) (exponent_m | exponent_v << 8);
+  const Part<T> part(t, factor, rates);
+  const int64_t block = part.first / kBlock + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (block * kBlock >= part.count) return;  // the whole wavefront
+  if (part.aligned && (block + 1) * kBlock <= part.count) adamw8_block<T, kStream, true>(part, s, block);
+  else adamw8_block<T, kStream, false>(part, s, block);
 }
 
 struct MomentsTable {
@@ -328,12 +358,11 @@ __global__ void __launch_bounds__(256) adamw8_pack_kernel(MomentsTable t) {
   if (block * kBlock >= t.count[q]) return;
   const int64_t e = block * kBlock + lane * 4, left = t.count[q] - e;
   const StateView state = view_state(t.state[q], t.count[q]);
-  float m[4], v[4];
-  load4<false>((const float*) t.m[q] + e, left, false, m), load4<false>((const float*) t.v[q] + e, left, false, v);
+  const Four<float> m = load4<false, false>((const float*) t.m[q] + e, left), v = load4<false, false>((const float*) t.v[q] + e, left);
   const uint32_t noise[4] = {0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
   uint32_t codes_m, codes_v;
   int exponent_m, exponent_v;
-  encode4(m, v, noise, codes_m, codes_v, exponent_m, exponent_v);
+  encode4(m.x, v.x, noise, codes_m, codes_v, exponent_m, exponent_v);
   *(uint32_t*) (state.m + e) = codes_m, *(uint32_t*) (state.v + e) = codes_v;
   if (lane == 0) *(uint16_t*) (state.exponents + 2 * block) = (uint16_t) (exponent_m | exponent_v << 8);
 }
@@ -366,14 +395,20 @@ __global__ void __launch_bounds__(256) square_sums_kernel(NormTable t, double* _
     const T* grad = (const T*) t.grad[q];
     const bool aligned = ((uintptr_t) grad & (4 * sizeof(T) - 1)) == 0;
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (aligned && (int64_t) (chunk - t.first_chunk[q] + 1) * kNormChunk <= count) {
+      Four<T> g[kNormChunk / 1024];
 #pragma unroll
-    for (int j = 0; j < kNormChunk / 1024; ++j) {
-      const int64_t e = at + j * 1024;
-      if (e >= count) break;
-      float g[4];
-      load4<kStream>(grad + e, count - e, aligned && count - e >= 4, g);
+      for (int j = 0; j < kNormChunk / 1024; ++j) g[j] = load4<true, kStream>(grad + at + j * 1024, 4);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) sum[k] = fmaf(g[k], g[k], sum[k]);
+      for (int j = 0; j < kNormChunk / 1024; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[k] = fmaf(to_float(g[j].x[k]), to_float(g[j].x[k]), sum[k]);
+    } else {
+      for (int64_t e = at; e < count && e < at + kNormChunk; e += 1024) {
+        const Four<T> g = load4<false, kStream>(grad + e, count - e);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[k] = fmaf(to_float(g.x[k]), to_float(g.x[k]), sum[k]);
+      }
     }
     total += ((double) sum[0] + sum[1]) + ((double) sum[2] + sum[3]);
   }
