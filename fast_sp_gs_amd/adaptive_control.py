@@ -19,6 +19,7 @@ import torch
 from torch import Tensor, nn
 
 from ._C import get_C_function
+from .adamw import adamw8_moments, adamw8_pack, adamw8_state
 
 
 def inverse_sigmoid(x: Tensor) -> Tensor:
@@ -36,7 +37,8 @@ def restructure_optimizer(optimizers, names: Sequence[str], source_row: Tensor, 
     New parameter = old[source_row]; the last `new_rows` rows are new points: their moments are zero (the reference
     concatenates `zeros_like`, gaussian_splatting.py:539-543); where `tail[name]` is given, the last `len(tail[name])`
     parameter rows are taken from it instead of from the table. Returns {group name: new nn.Parameter}, as `change_optimizer` does
-    (gaussian_splatting.py:497-555).
+    (gaussian_splatting.py:497-555). 8-bit moments (`AdamW(state_bits=8)`) lie in blocks that follow the memory, not the rows: they are
+    gathered as values and packed again.
     """
     gather = get_C_function('gather_rows')
     tail = tail or {}
@@ -56,6 +58,8 @@ def restructure_optimizer(optimizers, names: Sequence[str], source_row: Tensor, 
             params.append(old)
             if state is not None and 'exp_avg' in state:
                 moments += [state['exp_avg'], state['exp_avg_sq']]
+            elif state is not None and 'moments8' in state:
+                moments += adamw8_moments([state['moments8']], [old.detach()])[0]
     if moment_row is source_row:  # no new rows: parameters and moments follow the same table, one launch
         both = gather(params + moments, source_row)
         new_params, new_moments = both[:len(params)], both[len(params):]
@@ -75,6 +79,9 @@ def restructure_optimizer(optimizers, names: Sequence[str], source_row: Tensor, 
         del optimizer.state[old]
         if 'exp_avg' in state:
             state['exp_avg'], state['exp_avg_sq'] = new_moments[k], new_moments[k + 1]
+            k += 2
+        elif 'moments8' in state:
+            state['moments8'], = adamw8_pack([new_moments[k]], [new_moments[k + 1]])
             k += 2
         optimizer.state[new] = state
     return out
@@ -258,6 +265,8 @@ class AdaptiveControl:
                     if 'exp_avg' in state:
                         state['exp_avg'] = torch.zeros_like(new)
                         state['exp_avg_sq'] = torch.zeros_like(new)
+                    elif 'moments8' in state:
+                        state['moments8'] = adamw8_state(new)
                     opt.state[new] = state
                 self._opacity = new
 

@@ -7,9 +7,13 @@ Gaussians, Adam on the network and the control points.
 `DynamicStep` owns the state (parameters, the two optimisers); `forward_loss` is the differentiable part alone so that
 tests can compare its gradients with other formulations.
 
-The network runs on the bf16 copies of its weights that it made when it was first called, since the network's optimiser
+With neighbour logits `sp_W` [N, M] (LBS_method 'W', network.py:514-515) the association of points to control points is learned too, held
+apart by `balance` times the balance loss of the logits; `weight_decay`, `state_bits` and `max_norm` have the network, the control points
+and the logits stepped by `AdamW` instead of plain Adam.
+
+The network runs on the bf16 copies of its weights that it made when it was first called, since the network's plain optimiser
 leaves the parameters' version counters alone, as torch's fused Adam does: a training loop calls `step.net.pack()` after
-each step to have the stepped weights in use.
+each step to have the stepped weights in use. `AdamW` advances the counters, and the network packs anew by itself.
 """
 from __future__ import annotations
 
@@ -18,6 +22,8 @@ from typing import Optional
 import torch
 from torch import Tensor
 
+from fast_sp_gs_amd.adamw import AdamW
+from fast_sp_gs_amd.balance import balance_loss
 from fast_sp_gs_amd.deform import _FUSED_WARPS, DeformNetwork, _fused_deform, deform_apply, superpoint_deform
 from fast_sp_gs_amd.renderer import GS_2D_render
 from fast_sp_gs_amd.sparse_gaussian_adam import DenseAdam, SparseGaussianAdam
@@ -32,7 +38,8 @@ class DynamicStep:
     def __init__(self, scene, cam, control_points: Tensor, target: Tensor, K: int = 4, temperature: float = 0.01,
                  local_frame: bool = True, warp_method: str = 'LBS', LBS_method: str = 'dist', lr: float = 1.6e-4,
                  net_lr: float = 1e-7, lambda_dssim: float = 0.2, background: Optional[Tensor] = None,
-                 net: Optional[DeformNetwork] = None):
+                 net: Optional[DeformNetwork] = None, sp_W: Optional[Tensor] = None, association_lr: float = 1e-3,
+                 balance: float = 0.0, weight_decay: float = 0.0, state_bits: int = 32, max_norm: Optional[float] = None):
         dev = scene.means3D.device
         self.cam, self.target, self.K, self.temperature = cam, target, K, temperature
         self.warp_method, self.LBS_method, self.lambda_dssim = warp_method, LBS_method, lambda_dssim
@@ -42,7 +49,17 @@ class DynamicStep:
         self.params = [getattr(scene, k).detach().clone().requires_grad_(True) for k in PARAM_NAMES]
         self.opt = SparseGaussianAdam([{'params': [p], 'name': k} for p, k in zip(self.params, PARAM_NAMES)], lr=lr,
                                       eps=1e-15)
-        self.net_opt = DenseAdam(list(self.net.parameters()) + [self.ctrl], lr=net_lr)
+        if (sp_W is None) == (LBS_method == 'W') or (balance and sp_W is None):
+            raise ValueError("neighbour logits sp_W go with LBS_method 'W', and a balance with them")
+        self.sp_W, self.balance = None if sp_W is None else sp_W.detach().clone().requires_grad_(True), balance
+        learned = list(self.net.parameters()) + [self.ctrl]
+        if sp_W is None and not weight_decay and state_bits == 32 and max_norm is None:
+            self.net_opt = DenseAdam(learned, lr=net_lr)
+        else:
+            groups = [{'params': learned, 'lr': net_lr}]
+            if sp_W is not None:  # decay would pull all of a point's logits together
+                groups.append({'params': [self.sp_W], 'lr': association_lr, 'weight_decay': 0.0, 'name': 'sp_W'})
+            self.net_opt = AdamW(groups, weight_decay=weight_decay, state_bits=state_bits, max_norm=max_norm)
         self.sh_degree = scene.sh_degree
         # the reference's training render passes `accum_max_count` on every step (network.py:706): per Gaussian, the
         # number of (pixel, blended entry) events at which it was the pixel's strongest contributor so far
@@ -50,7 +67,8 @@ class DynamicStep:
         self._one = torch.ones((), device=dev)  # the loss's own gradient, which backward() would fill a new tensor with each time
 
     def forward_loss(self, t: Tensor):
-        """-> (loss, render outputs). Differentiable in the Gaussians' parameters, the control points and the network."""
+        """-> (loss, render outputs). Differentiable in the Gaussians' parameters, the control points, the network and
+        the neighbour logits."""
         means3D, scales, rotations, opacities, shs = self.params
         c_xyz, c_rot, c_scale, c_local = self.net(self.ctrl.detach(), t)
         columns = scales.shape[1]
@@ -62,13 +80,16 @@ class DynamicStep:
         else:
             d_xyz, d_rot, d_scale, _, _ = superpoint_deform(
                 means3D.detach(), self.ctrl, c_xyz, c_rot, c_scale[:, :columns], sp_rot=c_local, K=self.K,
-                temperature=self.temperature, warp_method=self.warp_method, LBS_method=self.LBS_method)
+                temperature=self.temperature, warp_method=self.warp_method, LBS_method=self.LBS_method, sp_W=self.sp_W)
         xyz, sc, rot = deform_apply(means3D, d_xyz, scales, d_scale, rotations, d_rot)
         cam = self.cam
         out = GS_2D_render(xyz, sc, rot, opacities, (cam.W, cam.H), cam.Tw2v, cam.Tv2c, campos=cam.campos,
                            near=cam.near, far=cam.far, sh_degree=self.sh_degree, sh_features=shs,
                            background=self.background, accum_max_count=self.accum_max_count)
-        return l1_dssim_loss(out['images'], self.target, self.lambda_dssim), out
+        loss = l1_dssim_loss(out['images'], self.target, self.lambda_dssim)
+        if self.balance:
+            loss = loss + self.balance * balance_loss(self.sp_W, 1)[0]
+        return loss, out
 
     def step(self, t: Tensor):
         """One full iteration; returns (loss, visibility mask) as device tensors (nothing is copied to the host)."""
