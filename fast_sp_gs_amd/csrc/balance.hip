@@ -102,6 +102,9 @@ __device__ __forceinline__ int column(int lane, int j) {
   constexpr int kPiece = 16 / sizeof(T);
   return (j / kPiece * kLanes + lane) * kPiece + j % kPiece;
 }
+// How logits are read: element by element; in pieces, which are aligned and end where the row ends; in pieces past the caches.
+enum Access { kSingle, kWhole, kStream };
+
 // A lane's part of a row as it lies in memory. A row that is not `on` is read where the first one is, a column that there is not where the
 // row begins: no branch stands between the loads, so that they stay in flight while the row before is worked on.
 template <typename T, int kLanes, int kVals>
@@ -109,19 +112,22 @@ struct Row {
   static constexpr int kPiece = 16 / sizeof(T);
   Pack<T, kPiece> piece[kVals / kPiece];
 
-  template <bool kWhole>  // pieces are aligned, and end where the row ends
+  template <Access kAccess>
   __device__ __forceinline__ void load(const T* __restrict__ row, int M, int lane) {
 #pragma unroll
     for (int i = 0; i < kVals / kPiece; ++i) {
       const int c = column<T, kLanes>(lane, i * kPiece);
-      if (kWhole) piece[i] = *(const Pack<T, kPiece>*) (row + (c < M ? c : 0));
+      typedef uint32_t Raw __attribute__((ext_vector_type(4)));
+      if (kAccess == kStream)
+        piece[i] = __builtin_bit_cast(Pack<T, kPiece>, __builtin_nontemporal_load((const Raw*) (row + (c < M ? c : 0))));
+      else if (kAccess == kWhole) piece[i] = *(const Pack<T, kPiece>*) (row + (c < M ? c : 0));
       else
 #pragma unroll
         for (int k = 0; k < kPiece; ++k) piece[i].x[k] = row[c + k < M ? c + k : 0];
     }
   }
   // -inf for what there is not; `full`: every lane has kVals columns
-  template <bool kWhole>
+  template <Access kAccess>
   __device__ __forceinline__ void values(float x[kVals], int M, bool full, bool on, int lane) const {
 #pragma unroll
     for (int j = 0; j < kVals; ++j) x[j] = to_float(piece[j / kPiece].x[j % kPiece]);
@@ -135,7 +141,7 @@ struct Row {
     for (int i = 0; i < kVals; i += kPiece) {
       if ((i / kPiece + 1) * kLanes * kPiece <= M) continue;  // of all lanes
 #pragma unroll
-      for (int k = 0; k < kPiece; ++k) x[i + k] = column<T, kLanes>(l, i + (kWhole ? 0 : k)) < M ? x[i + k] : -INFINITY;
+      for (int k = 0; k < kPiece; ++k) x[i + k] = column<T, kLanes>(l, i + (kAccess == kSingle ? k : 0)) < M ? x[i + k] : -INFINITY;
     }
   }
 };
@@ -206,8 +212,8 @@ __device__ __forceinline__ void choose(const float x[kVals], int lane_top, int t
   for (int j = 0; j < kVals; ++j) count[j] += x[j] >= t ? 1 : 0;
 }
 
-template <typename T, int kLanes, int kVals, bool kWhole>
-__global__ void __launch_bounds__(row_threads(kVals), row_waves(kVals, sizeof(T) == 2 && kWhole)) balance_rows_kernel(int64_t N, int M, int64_t ld, int K,
+template <typename T, int kLanes, int kVals, Access kAccess>
+__global__ void __launch_bounds__(row_threads(kVals), row_waves(kVals, sizeof(T) == 2 && kAccess != kSingle)) balance_rows_kernel(int64_t N, int M, int64_t ld, int K,
     const T* __restrict__ logits, const uint8_t* __restrict__ rows, float2* __restrict__ stats, float* __restrict__ sums,
     int* __restrict__ counts, BlockRows* __restrict__ blocks, unsigned* __restrict__ ticket) {
   constexpr int kRows = 64 / kLanes, kThreads = row_threads(kVals), kWaves = kThreads / 64;
@@ -232,7 +238,7 @@ __global__ void __launch_bounds__(row_threads(kVals), row_waves(kVals, sizeof(T)
   auto address = [&](int64_t row, bool on) { return logits + (on ? row : 0) * ld; };
   auto work = [&](const Row<T, kLanes, kVals>& row, int64_t at, bool on) {
     float x[kVals];
-    row.template values<kWhole>(x, M, full, on, lane);
+    row.template values<kAccess>(x, M, full, on, lane);
     float lane_top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < kVals; ++j) lane_top = fmaxf(lane_top, x[j]);
@@ -256,16 +262,16 @@ __global__ void __launch_bounds__(row_threads(kVals), row_waves(kVals, sizeof(T)
   Row<T, kLanes, kVals> a, b;
   bool on_a = on_of(base + group, mask_of(base + group)), on_b;
   int mask = mask_of(base + step + group);
-  a.template load<kWhole>(address(base + group, on_a), M, lane);
+  a.template load<kAccess>(address(base + group, on_a), M, lane);
   for (; base < N; base += 2 * step) {
     const int64_t at = base + group;
     on_b = on_of(at + step, mask);
     mask = mask_of(at + 2 * step);
-    b.template load<kWhole>(address(at + step, on_b), M, lane);
+    b.template load<kAccess>(address(at + step, on_b), M, lane);
     work(a, at, on_a);
     on_a = on_of(at + 2 * step, mask);
     mask = mask_of(at + 3 * step);
-    a.template load<kWhole>(address(at + 2 * step, on_a), M, lane);
+    a.template load<kAccess>(address(at + 2 * step, on_a), M, lane);
     if (base + step < N) work(b, at + step, on_b);
   }
   // the rows' groups of a wavefront, then the wavefronts one after the other
@@ -296,8 +302,8 @@ __global__ void __launch_bounds__(row_threads(kVals), row_waves(kVals, sizeof(T)
   }
 }
 
-// kWhole: also of the gradient's rows
-template <typename T, int kLanes, int kVals, bool kWhole>
+// the access also of the gradient's rows
+template <typename T, int kLanes, int kVals, Access kAccess>
 __global__ void __launch_bounds__(256) balance_rows_backward_kernel(int64_t N, int M, int64_t ld, const T* __restrict__ logits,
     const float2* __restrict__ stats, const int* __restrict__ counts, const int64_t* __restrict__ totals,
     const float* __restrict__ g_loss, const float* __restrict__ g_importance, T* __restrict__ grad) {
@@ -323,7 +329,7 @@ __global__ void __launch_bounds__(256) balance_rows_backward_kernel(int64_t N, i
   auto work = [&](const Row<T, kLanes, kVals>& row, int64_t at, float2 stat) {
     const bool on = on_of(at, stat);
     float x[kVals], mean = 0.0f;
-    row.template values<kWhole>(x, M, full, on, lane);
+    row.template values<kAccess>(x, M, full, on, lane);
 #pragma unroll
     for (int j = 0; j < kVals; ++j) {
       x[j] = __builtin_amdgcn_exp2f((x[j] - stat.x) * kLog2e) * stat.y;
@@ -338,7 +344,10 @@ __global__ void __launch_bounds__(256) balance_rows_backward_kernel(int64_t N, i
       Pack<T, kPiece> q;
 #pragma unroll
       for (int k = 0; k < kPiece; ++k) from_float(x[j + k] * (slope[j + k] - mean), q.x[k]);
-      if (kWhole) {
+      if (kAccess == kStream) {
+        typedef uint32_t Raw __attribute__((ext_vector_type(4)));
+        if (c < M) __builtin_nontemporal_store(__builtin_bit_cast(Raw, q), (Raw*) (out + c));
+      } else if (kAccess == kWhole) {
         if (c < M) *(Pack<T, kPiece>*) (out + c) = q;
       } else {
 #pragma unroll
@@ -349,14 +358,14 @@ __global__ void __launch_bounds__(256) balance_rows_backward_kernel(int64_t N, i
   };
   Row<T, kLanes, kVals> a, b;
   float2 stat_a = stat_of(base + group), stat_b = stat_of(base + step + group), after;
-  a.template load<kWhole>(address(base + group, on_of(base + group, stat_a)), M, lane);
+  a.template load<kAccess>(address(base + group, on_of(base + group, stat_a)), M, lane);
   for (; base < N; base += 2 * step) {
     const int64_t at = base + group;
     after = stat_of(at + 2 * step);
-    b.template load<kWhole>(address(at + step, on_of(at + step, stat_b)), M, lane);
+    b.template load<kAccess>(address(at + step, on_of(at + step, stat_b)), M, lane);
     work(a, at, stat_a);
     stat_a = after, after = stat_of(at + 3 * step);
-    a.template load<kWhole>(address(at + 2 * step, on_of(at + 2 * step, stat_a)), M, lane);
+    a.template load<kAccess>(address(at + 2 * step, on_of(at + 2 * step, stat_a)), M, lane);
     if (base + step < N) work(b, at + step, stat_b);
     stat_b = after;
   }
@@ -681,6 +690,9 @@ int neighbour_blocks(int64_t N) {
   return (int) (blocks < kNeighbourBlocks ? blocks : kNeighbourBlocks);
 }
 
+// Logits that exceed the 256 MB memory-side cache are read past it.
+bool past_caches(int64_t N, int M, size_t size) { return N >= ((int64_t) 160 << 20) / (int64_t) (M * size); }
+
 // kernel<T, lanes, values>(...) for the narrowest rows that hold M columns
 #define FSGS_ROW_KERNELS(T, LAUNCH)                         \
   do {                                                      \
@@ -705,9 +717,11 @@ void launch_rows(int G, int64_t N, int M, int64_t ld, int K, const void* logits,
     return;
   }
   const bool whole = M % (16 / sizeof(T)) == 0 && ld * sizeof(T) % 16 == 0 && (uintptr_t) logits % 16 == 0;
-#define LAUNCH(T, L, V)                                                                                                          \
-  hipLaunchKernelGGL((whole ? balance_rows_kernel<T, L, V, true> : balance_rows_kernel<T, L, V, false>), dim3(G), dim3(row_threads(V)), 0, \
-                     s, N, M, ld, K, x, rows, stats, sums, counts, blocks, ticket)
+#define LAUNCH(T, L, V)                                                                                                               \
+  hipLaunchKernelGGL((!whole ? balance_rows_kernel<T, L, V, kSingle>                                                                  \
+                      : past_caches(N, M, sizeof(T)) ? balance_rows_kernel<T, L, V, V < 32 ? kStream : kWhole>                        \
+                                                     : balance_rows_kernel<T, L, V, kWhole>),                                         \
+                     dim3(G), dim3(row_threads(V)), 0, s, N, M, ld, K, x, rows, stats, sums, counts, blocks, ticket)
   FSGS_ROW_KERNELS(T, LAUNCH);
 #undef LAUNCH
 }
@@ -724,8 +738,10 @@ void launch_rows_backward(int G, int64_t N, int M, int64_t ld, const void* logit
   }
   const bool whole = M % (16 / sizeof(T)) == 0 && ld * sizeof(T) % 16 == 0 && ((uintptr_t) logits | (uintptr_t) grad) % 16 == 0;
 #define LAUNCH(T, L, V)                                                                                                             \
-  hipLaunchKernelGGL((whole ? balance_rows_backward_kernel<T, L, V, true> : balance_rows_backward_kernel<T, L, V, false>), dim3(G), \
-                     dim3(256), 0, s, N, M, ld, x, stats, counts, totals, g_loss, g_importance, out)
+  hipLaunchKernelGGL((!whole ? balance_rows_backward_kernel<T, L, V, kSingle>                                                       \
+                      : past_caches(N, M, sizeof(T)) ? balance_rows_backward_kernel<T, L, V, V < 32 ? kStream : kWhole>             \
+                                                     : balance_rows_backward_kernel<T, L, V, kWhole>),                              \
+                     dim3(G), dim3(256), 0, s, N, M, ld, x, stats, counts, totals, g_loss, g_importance, out)
   FSGS_ROW_KERNELS(T, LAUNCH);
 #undef LAUNCH
 }

@@ -58,14 +58,6 @@ struct Launches {
   }
 };
 
-// A tensor of its own over a part of an allocation, laid out as `like`.
-Tensor part_of(const Tensor& all, int64_t offset, const Tensor& like) {
-  auto part = c10::make_intrusive<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(all.storage()), all.key_set(), all.dtype());
-  part->set_storage_offset(offset);
-  part->set_sizes_and_strides(like.sizes(), like.strides());
-  return Tensor(std::move(part));
-}
-
 template <typename T, typename F>
 std::vector<T> pick(const std::vector<size_t>& which, F of) {
   std::vector<T> out;
@@ -251,14 +243,15 @@ std::vector<std::pair<Tensor, Tensor>> adamw8_moments(const std::vector<Tensor>&
   }
   const c10::DeviceGuard guard(device);
   // parts of one allocation, each on a boundary of its own: an allocation for every one of 50 tensors took 40 us
-  const auto room = [](const Tensor& t) { return (t.numel() + 255) / 256 * 256; };
+  const int64_t size = type == at::kFloat ? 4 : 2;
+  const auto room = [&](const Tensor& t) { return (t.numel() * size + 511) / 512 * 512; };
   int64_t total = 0;
   for (const Tensor& t : like) total += 2 * room(t);
-  const Tensor all = empty({total}, states[0], type);
+  const Tensor all = empty({total}, states[0], at::kByte);
   int64_t at = 0;
   for (const Tensor& t : like) {
-    const Tensor m = part_of(all, at, t), v = part_of(all, at + room(t), t);
-    out.push_back({m, v}), at += 2 * room(t);
+    const auto part = [&](int64_t from) { return part_of(all, from, t.sizes(), t.strides(), type); };
+    out.push_back({part(at), part(at + room(t))}), at += 2 * room(t);
   }
   const size_t n = states.size(), most = (size_t) fsgs_adamw_max_tensors();
   for (size_t from = 0; from < n; from += most) {

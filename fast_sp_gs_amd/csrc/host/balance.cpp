@@ -7,10 +7,16 @@
 namespace fsgs_host {
 namespace {
 
+// The results in one allocation, what the backward reads besides them in another: [2] totals, then `extra` bytes.
 struct Outputs {
-  Tensor loss, counts, importance, totals;
-  Outputs(int64_t M, const Tensor& like)
-      : loss(empty({}, like)), counts(empty({M}, like, at::kInt)), importance(empty({M}, like)), totals(empty({2}, like, at::kLong)) {}
+  Tensor loss, counts, importance, saved;
+  Outputs(int64_t M, const Tensor& like, int64_t extra = 0) : saved(empty({16 + extra}, like, at::kByte)) {
+    const Tensor all = empty({16 + 8 * M}, like, at::kByte);
+    loss = part_of(all, 0, {}, {}, at::kFloat), importance = part_of(all, 16, {M}, {1}, at::kFloat);
+    counts = part_of(all, 16 + 4 * M, {M}, {1}, at::kInt);
+  }
+  int64_t* totals() const { return data<int64_t>(saved); }
+  float* stats() const { return (float*) (data<uint8_t>(saved) + 16); }
 };
 
 int logits_code(at::ScalarType type) {
@@ -37,14 +43,14 @@ Tensor rows_of(const Tensor& logits) {
 }
 int64_t stride_of(const Tensor& logits) { return logits.size(0) > 1 ? logits.stride(0) : logits.size(1); }
 
-Outputs rows_forward(const Tensor& logits, int64_t K, const Tensor& rows, const Tensor& stats) {
+Outputs rows_forward(const Tensor& logits, int64_t K, const Tensor& rows, bool train) {
   const int64_t N = logits.size(0), M = logits.size(1);
   const int code = logits_code(logits.scalar_type());
-  Outputs out(M, logits);
+  Outputs out(M, logits, train ? 8 * N : 0);
   const size_t bytes = fsgs_balance_loss_workspace_bytes(N, (int) M, code);
   const Tensor ws = empty({(int64_t) bytes}, logits, at::kByte);
   check(fsgs_balance_loss_forward(N, (int) M, stride_of(logits), (int) K, code, logits.data_ptr(), data<uint8_t>(rows), f32(out.loss),
-                                  i32(out.counts), f32(out.importance), i64(out.totals), f32(stats), ws.data_ptr(), bytes, stream_of(logits)),
+                                  i32(out.counts), f32(out.importance), out.totals(), train ? out.stats() : nullptr, ws.data_ptr(), bytes, stream_of(logits)),
         "balance_loss");
   return out;
 }
@@ -55,7 +61,7 @@ Outputs neighbours_forward(const Tensor& weights, const Tensor& indices, int64_t
   const size_t bytes = fsgs_neighbour_balance_workspace_bytes(N, (int) M);
   const Tensor ws = empty({(int64_t) bytes}, weights, at::kByte);
   check(fsgs_neighbour_balance_forward(N, (int) M, (int) K, f32(weights), i64(indices), data<uint8_t>(rows), f32(out.loss), i32(out.counts),
-                                       f32(out.importance), i64(out.totals), ws.data_ptr(), bytes, stream_of(weights)),
+                                       f32(out.importance), out.totals(), ws.data_ptr(), bytes, stream_of(weights)),
         "neighbour_balance");
   return out;
 }
@@ -73,9 +79,8 @@ struct Upstream {
 
 struct RowsNode : public torch::autograd::Function<RowsNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, int64_t K, const OptTensor& rows) {
-    const Tensor stats = empty({logits.size(0), 2}, logits);
-    const Outputs out = rows_forward(logits, K, opt(rows), stats);
-    ctx->save_for_backward({logits, stats, out.totals, out.counts});
+    const Outputs out = rows_forward(logits, K, opt(rows), true);
+    ctx->save_for_backward({logits, out.saved, out.counts});
     ctx->mark_non_differentiable({out.counts});
     ctx->set_materialize_grads(false);
     return {out.loss, out.counts, out.importance};
@@ -87,13 +92,13 @@ struct RowsNode : public torch::autograd::Function<RowsNode> {
     const auto t = ctx->get_saved_variables();
     at::AutoDispatchBelowADInplaceOrView no_graph;
     const Tensor logits = rows_of(t[0]);  // a hook may hand it back in another layout
-    const Tensor &stats = t[1], &totals = t[2], &counts = t[3];
+    const Tensor &saved = t[1], &counts = t[2];
     const c10::DeviceGuard guard(logits.device());
     up.check_types(what);
     const Tensor grad = at::empty(logits.sizes(), logits.options());
     if (grad.numel() > 0)
       check(fsgs_balance_loss_backward(logits.size(0), (int) logits.size(1), stride_of(logits), logits_code(logits.scalar_type()),
-                                       logits.data_ptr(), f32(stats), i32(counts), i64(totals), f32(up.loss), f32(up.importance),
+                                       logits.data_ptr(), (const float*) (data<uint8_t>(saved) + 16), i32(counts), data<int64_t>(saved), f32(up.loss), f32(up.importance),
                                        grad.data_ptr(), stream_of(logits)),
             what);
     return first_order_only(g, {t[0]}, {grad, Tensor(), Tensor()});
@@ -103,7 +108,7 @@ struct RowsNode : public torch::autograd::Function<RowsNode> {
 struct NeighboursNode : public torch::autograd::Function<NeighboursNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& weights, const Tensor& indices, int64_t M, const OptTensor& rows) {
     const Outputs out = neighbours_forward(weights, indices, M, opt(rows));
-    ctx->save_for_backward({indices, opt(rows), out.totals, out.counts});
+    ctx->save_for_backward({indices, opt(rows), out.saved, out.counts});
     ctx->saved_data["M"] = M;
     ctx->mark_non_differentiable({out.counts});
     ctx->set_materialize_grads(false);
@@ -116,13 +121,13 @@ struct NeighboursNode : public torch::autograd::Function<NeighboursNode> {
     const auto t = ctx->get_saved_variables();
     at::AutoDispatchBelowADInplaceOrView no_graph;
     const Tensor indices = t[0].contiguous(), rows = contiguous(t[1]);
-    const Tensor &totals = t[2], &counts = t[3];
+    const Tensor &saved = t[2], &counts = t[3];
     const c10::DeviceGuard guard(indices.device());
     up.check_types(what);
-    const Tensor grad = empty(indices.sizes(), totals);
+    const Tensor grad = empty(indices.sizes(), saved);
     if (grad.numel() > 0)
       check(fsgs_neighbour_balance_backward(indices.size(0), (int) ctx->saved_data["M"].toInt(), (int) indices.size(1), i64(indices),
-                                            data<uint8_t>(rows), i32(counts), i64(totals), f32(up.loss), f32(up.importance), f32(grad),
+                                            data<uint8_t>(rows), i32(counts), data<int64_t>(saved), f32(up.loss), f32(up.importance), f32(grad),
                                             stream_of(indices)),
             what);
     return first_order_only(g, {}, {grad, Tensor(), Tensor(), Tensor()});
@@ -147,7 +152,7 @@ std::tuple<Tensor, Tensor, Tensor> balance_loss(const Tensor& logits, int64_t K,
     const variable_list out = RowsNode::apply(x, K, given(on));
     return {out[0], out[1], out[2]};
   }
-  const Outputs out = rows_forward(x, K, on, Tensor());
+  const Outputs out = rows_forward(x, K, on, false);
   return {out.loss, out.counts, out.importance};
 }
 
