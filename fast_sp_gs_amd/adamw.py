@@ -3,7 +3,7 @@ norm of all of them together. No counterpart in the reference, whose optimisers 
 networks are regularised by decay, and where learned neighbour logits `sp_W[N, M]` (LBS_method 'W') make the optimiser's moments the
 largest thing in memory: 8 bytes an element in 32 bits, 2 in 8.
 
-    m = b1 m + (1 - b1) c g,  v = b2 v + (1 - b2) (c g)^2,  c = min(1, max_norm / (|g| + 1e-6))
+    m = b1 m + (1 - b1) c g,  v = b2 v + (1 - b2) (c g)^2,  c = min(1, max_norm / (|g| + 1e-6)), NaN if |g| is
     p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 
 `adamw_step` and `adamw8_step` step lists of tensors, `AdamW` is the optimiser class over them. Parameters and gradients are float32,
@@ -31,7 +31,7 @@ Rate = Union[float, Sequence[float]]
 
 def _each(value: Rate, n: int) -> List[float]:
     """A number for all tensors, or one for each of them."""
-    return [float(value)] * n if isinstance(value, (int, float)) else [float(v) for v in value]
+    return [float(v) for v in value] if isinstance(value, (list, tuple)) else [float(value)] * n
 
 
 def grad_norm(grads: Sequence[Tensor], max_norm: float = float('inf')) -> Tensor:
@@ -91,7 +91,8 @@ class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's step on the kernels above. `state_bits` 32: states as torch's AdamW keeps them (checkpoints load either way),
     float32 for parameters of any type; 8: `moments8`, the uint8 state (32-bit checkpoints are taken over, and the other way round).
     `max_norm` clips the gradients by the norm of all of them together within the step, without writing them; `last_norm` then holds that norm.
-    `capturable` keeps the step counts on the device, for steps captured into a graph; rates are captured as they are. The step tells autograd that
+    `capturable` keeps the step counts on the device, for steps captured into a graph (after a first one that is not); rates are captured as
+    they are. The step tells autograd that
     the parameters changed, so `DeformNetwork` packs its weights anew by itself."""
 
     def __init__(self, params, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
@@ -106,9 +107,14 @@ class AdamW(torch.optim.Optimizer):
         self.state_bits, self.max_norm, self.seed, self.last_norm = state_bits, max_norm, seed, None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, capturable=capturable))
 
+    def __getstate__(self):  # torch keeps the groups and the states alone
+        return dict(super().__getstate__(), state_bits=self.state_bits, max_norm=self.max_norm, seed=self.seed, last_norm=None)
+
     def _state_of(self, p: Tensor, capturable: bool):
         state = self.state[p]
         if not state:
+            if torch.cuda.is_current_stream_capturing():  # every replay would start from zero again
+                raise RuntimeError('AdamW: take one step before a step is captured')
             state['step'] = torch.zeros((), dtype=torch.float32, device=p.device if capturable else 'cpu')
             if self.state_bits == 8:
                 state['moments8'] = adamw8_state(p)
@@ -151,6 +157,8 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """Also a checkpoint with moments of the other width. torch casts what it loads to the parameter's type, which moments do not
         have here: they are taken from the checkpoint itself."""
+        if any(group.get('amsgrad') or group.get('maximize') for group in state_dict['param_groups']):
+            raise ValueError('AdamW: checkpoints of amsgrad or maximize steps cannot be taken over')
         super().load_state_dict(state_dict)
         ids = chain.from_iterable(group['params'] for group in state_dict['param_groups'])
         own = [(p, group['capturable']) for group in self.param_groups for p in group['params']]

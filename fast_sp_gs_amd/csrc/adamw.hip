@@ -543,6 +543,8 @@ int adamw_update(const char* what, int bits, int n, int dtype, const int64_t* co
   AdamwTable t{};
   if (const int rc = lay_out(what, t, t.first_block, n, count, 1024)) return rc;
   if (t.first_block[n] == 0) return kOk;
+  double known = 0.0, c1 = 1.0;
+  float inv_root_c2 = 1.0f;
   for (int q = 0; q < n; ++q) {
     const uintptr_t wide = (uintptr_t) m[q] | (v ? (uintptr_t) v[q] : 0), narrow = (uintptr_t) param[q] | (uintptr_t) grad[q];
     FSGS_REQUIRE(count[q] == 0 || (param[q] && grad[q] && m[q] && (!v || v[q]) && wide % (bits == 8 ? 16 : 4) == 0 && narrow % type_size(dtype) == 0),
@@ -551,9 +553,13 @@ int adamw_update(const char* what, int bits, int n, int dtype, const int64_t* co
     t.keep[q] = (float) (1.0 - lr[q] * decay[q]), t.eps[q] = (float) eps[q];
     if (rates) continue;
     FSGS_REQUIRE(step[q] >= 1.0, "%s: tensor %d has taken no step", what, q);
-    t.rates[q].step_size   = (float) (lr[q] / (1.0 - std::pow(b1, step[q])));
-    t.rates[q].inv_root_c2 = (float) (1.0 / std::sqrt(1.0 - std::pow(b2, step[q])));
-    t.rates[q].key         = noise_key((uint32_t) (int64_t) step[q], seed);
+    if (step[q] != known) {  // the tensors of a call mostly share their count, and powers take their time
+      known = step[q];
+      c1 = 1.0 - std::pow(b1, known), inv_root_c2 = (float) (1.0 / std::sqrt(1.0 - std::pow(b2, known)));
+    }
+    t.rates[q].step_size   = (float) (lr[q] / c1);
+    t.rates[q].inv_root_c2 = inv_root_c2;
+    t.rates[q].key         = noise_key((uint32_t) (int64_t) known, seed);
   }
   const Step s{(float) b1, (float) b2, (float) (1.0 - b1), (float) (1.0 - b2)};
   const bool past = streams(n, count, 3 * type_size(dtype) + (bits == 8 ? 4 : 16));

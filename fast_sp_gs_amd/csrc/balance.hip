@@ -16,6 +16,8 @@
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
+#include <algorithm>
+
 #include "../../include/fsgs.h"
 #include "common.hpp"
 
@@ -682,7 +684,9 @@ int pass_blocks(int64_t N, int M, int dtype) {
   if (N == 0) return 0;
   const int rows = M > kMostInLanes ? 1 : row_threads(M > 1024 ? 32 : 16) / lanes_of(M, dtype == FSGS_DTYPE_F32 ? 4 : 8);
   const int64_t blocks = (N + rows - 1) / rows;
-  return (int) (blocks < kRowBlocks ? blocks : kRowBlocks);
+  // sums and counts of M superpoints for each block: 256 MB of them at most, or what 32 blocks take
+  const int64_t most = std::min<int64_t>(kRowBlocks, std::max<int64_t>(32, ((int64_t) 1 << 25) / M));
+  return (int) std::min(blocks, most);
 }
 bool in_lds(int64_t M) { return M <= kMostInLds; }
 int neighbour_blocks(int64_t N) {

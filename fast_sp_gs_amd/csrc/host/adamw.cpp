@@ -32,8 +32,11 @@ bool alike(const Tensor& a, const Tensor& b) {
 
 void refuse_twice(const std::string& what, const char* name, const std::vector<Tensor>& list) {
   std::vector<const void*> at;
+  at.reserve(list.size());
+  bool rising = true;
   for (const Tensor& t : list)
-    if (t.numel() > 0) at.push_back(t.data_ptr());
+    if (t.numel() > 0) rising = rising && (at.empty() || at.back() < t.data_ptr()), at.push_back(t.data_ptr());
+  if (rising) return;
   std::sort(at.begin(), at.end());
   if (std::adjacent_find(at.begin(), at.end()) != at.end()) fail(what + ": a " + name + " is there twice");
 }
@@ -212,6 +215,7 @@ void adamw8_step(const std::vector<Tensor>& params, const std::vector<Tensor>& g
   for (size_t k = 0; k < params.size(); ++k) {
     require(what.c_str(), "state", states[k], at::kByte), require_device(what, "state", states[k], params[k].device());
     if (states[k].numel() != adamw8_state_bytes(params[k].numel())) fail(what + ": state " + number(k) + " is that of another number of elements");
+    if ((uintptr_t) states[k].data_ptr() % 16) fail(what + ": state " + number(k) + " must lie on a boundary of 16 bytes");
   }
   refuse_twice(what, "state", states);
   call.advance(steps);

@@ -443,3 +443,68 @@ def test_offsets_beyond_32_bits(device):
     adamw_step([p], [g], [ms], [vs], [torch.tensor(4.0)], 1e-2)
     _check_params(p[-far:], want, off, torch.bfloat16)
     assert not bool(ms[:-far].any())
+
+
+def test_first_step_is_not_captured(device):
+    """The states that a first step makes would be zeroed again by every replay."""
+    from fast_sp_gs_amd.adamw import AdamW
+    p = torch.nn.Parameter(torch.ones(10, device=device))
+    p.grad = torch.ones_like(p)
+    opt = AdamW([p], capturable=True)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match='before'):
+        with torch.cuda.graph(graph):
+            opt.step()
+
+
+def test_copies_and_pickles_of_the_optimiser(device):
+    import copy
+    import pickle
+    from fast_sp_gs_amd.adamw import AdamW
+    for make in (copy.deepcopy, lambda o: pickle.loads(pickle.dumps(o))):
+        p = torch.nn.Parameter(torch.linspace(0, 1, 600, device=device))
+        opt = AdamW([p], lr=1e-2, state_bits=8, max_norm=0.5, seed=3)
+        p.grad = torch.cos(p.detach())
+        opt.step()
+        other = make(opt)
+        q = other.param_groups[0]['params'][0]
+        for o, t in ((opt, p), (other, q)):
+            t.grad = torch.sin(t.detach())
+            o.step()
+        assert torch.equal(p.detach(), q.detach()) and float(other.last_norm) == float(opt.last_norm)
+
+
+def test_wrong_tensors_are_refused(device):
+    """Before anything is counted or written."""
+    from fast_sp_gs_amd.adamw import AdamW, adamw8_moments, adamw8_pack, adamw8_state, adamw8_step, adamw_step
+    p, step = torch.ones(8, device=device), torch.tensor(3.0)
+    ok = lambda: torch.zeros(8, device=device)
+    cases = [('there twice', dict(params=[p, p])), ('shape', dict(grads=[torch.ones(2, 4, device=device)])), ('dtype', dict(grads=[p.half()])),
+             ('differ', dict(m=[torch.zeros(4, 2, device=device)])), ('torch.float32', dict(m=[ok().half()])), ('one number', dict(steps=[torch.zeros(2)])),
+             ('CUDA', dict(grads=[torch.ones(8)])), ('gaps', dict(params=[torch.ones(16, device=device)[::2]])),
+             ('dtype', dict(params=[p.double()], grads=[p.double()])), ('there twice', dict(params=[ok(), ok()], m=[p, p])),
+             ('there twice', dict(params=[ok(), ok()], steps=[step, step]))]
+    for text, wrong in cases:
+        n = max(len(v) for v in wrong.values())
+        args = dict(params=[ok() for _ in range(n)], grads=[ok() for _ in range(n)], m=[ok() for _ in range(n)], v=[ok() for _ in range(n)],
+                    steps=[step.clone() for _ in range(n)])
+        args.update(wrong)
+        with pytest.raises(RuntimeError, match=text):
+            adamw_step(args['params'], args['grads'], args['m'], args['v'], args['steps'])
+        assert all(float(s.max()) in (0.0, 3.0) for s in args['steps'])
+    with pytest.raises(RuntimeError, match='all be on the host or all on the device'):
+        adamw_step([ok(), ok()], [ok(), ok()], [ok(), ok()], [ok(), ok()], [step, step.to(device)])
+    with pytest.raises(RuntimeError, match='another number of elements'):
+        adamw8_step([p], [p], [adamw8_state(torch.ones(300, device=device))], [step])
+    with pytest.raises(RuntimeError, match='another number of elements'):
+        adamw8_moments([adamw8_state(p)], [torch.ones(300, device=device)])
+    with pytest.raises(RuntimeError, match='uint8'):
+        adamw8_step([p], [p], [torch.zeros(514, device=device)], [step])
+    with pytest.raises(RuntimeError, match='boundary of 16 bytes'):
+        adamw8_step([p], [p], [torch.zeros(515, dtype=torch.uint8, device=device)[1:]], [step])
+    with pytest.raises(RuntimeError, match='differ'):
+        adamw8_pack([p], [p.view(2, 4)])
+    assert float(step) == 3.0 and torch.equal(p, torch.ones_like(p))
+    theirs = torch.optim.AdamW([torch.nn.Parameter(ok())], amsgrad=True)
+    with pytest.raises(ValueError, match='amsgrad'):
+        AdamW([torch.nn.Parameter(ok())]).load_state_dict(theirs.state_dict())

@@ -376,3 +376,44 @@ def test_training_of_an_association(device):
         moved = (sp_W.detach() - before).abs()
         assert bool(torch.isfinite(sp_W.detach()).all()) and 0 < float(moved.max()) <= 1e-2 * 7.3
     assert float(opt.state[sp_W]['step']) == 3.0
+
+
+def test_wrong_calls_are_refused(device):
+    from fast_sp_gs_amd.balance import balance_loss, neighbour_balance
+    x, w, i = torch.zeros(4, 5, device=device), torch.zeros(4, 2, device=device), torch.zeros(4, 2, dtype=torch.long, device=device)
+    for text, call in (('K must be', lambda: balance_loss(x, 0)), ('K must be', lambda: balance_loss(x, 6)),
+                       ('K must be', lambda: balance_loss(torch.zeros(4, 100, device=device), 65)), ('N, M', lambda: balance_loss(x[0], 1)),
+                       ('N, M', lambda: balance_loss(x[:, :0], 1)), ('dtype', lambda: balance_loss(x.double(), 1)),
+                       ('shape', lambda: balance_loss(x, 1, torch.ones(5, dtype=torch.bool, device=device))),
+                       ('torch.bool', lambda: balance_loss(x, 1, torch.ones(4, device=device))), ('CUDA', lambda: balance_loss(x, 1, torch.ones(4, dtype=torch.bool))),
+                       ('float32', lambda: neighbour_balance(w.half(), i, 3)), ('int64', lambda: neighbour_balance(w, i.int(), 3)),
+                       ('shape', lambda: neighbour_balance(w, i[:, :1], 3)), ('M must', lambda: neighbour_balance(w, i, 0)),
+                       ('N, K', lambda: neighbour_balance(w[0], i[0], 3)), ('shape', lambda: neighbour_balance(w, i, 3, torch.ones(3, dtype=torch.bool, device=device)))):
+        with pytest.raises(RuntimeError, match=text):
+            call()
+
+
+def test_two_threads_at_once(device):
+    """Calls of two host threads on streams of their own."""
+    import threading
+    g = torch.Generator(device=device).manual_seed(13)
+    sets = [(torch.randn(3000, 70 + 30 * k, generator=g, device=device), torch.softmax(torch.randn(3000, 3, generator=g, device=device), -1),
+             torch.randint(0, 70, (3000, 3), generator=g, device=device)) for k in range(2)]
+    run = lambda s: _both(s[0].clone().requires_grad_(True), s[1].clone().requires_grad_(True), s[2], 70, None)
+    want = [run(s) for s in sets]
+    torch.cuda.synchronize()
+    wrong = []
+    def work(k):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got = run(sets[k])
+                stream.synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[k])):
+                    wrong.append(k)
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
