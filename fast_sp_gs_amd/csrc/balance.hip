@@ -33,6 +33,7 @@ constexpr int kMostInLanes   = 4096;  // superpoints whose row is held by the la
 constexpr int kNeighbourBlocks = 256;
 constexpr int kNeighbourThreads = 1024;
 constexpr int kMostInLds     = 5400;  // superpoints whose sums (8 bytes) and counts (4) of a block fit in 64 KB beside a few words
+constexpr int kMostRanges    = 16;    // of so many superpoints, for each of which the weights are read again
 constexpr int kSlopeThreads  = 512;   // of their backward
 constexpr int kSlopeBlocks   = 1024;
 constexpr int kMostSlopes    = 8192;  // that it keeps in LDS
@@ -470,17 +471,20 @@ __global__ void __launch_bounds__(256) balance_wide_backward_kernel(int64_t N, i
 constexpr float kWeightUnits = 2147483648.0f;
 
 // A thread takes a row, four neighbours at a time: all loads of four are on their way before the first is looked at. kQuads: K is a
-// multiple of four and the addresses allow 16 bytes.
+// multiple of four and the addresses allow 16 bytes. A block keeps the superpoints of one range in LDS (blockIdx.y); beyond kMostRanges of
+// them the sums are global ones (kLds false). 3M points with 8 neighbours, us: 72 with 2048 superpoints, 109 if all are one and the same;
+// with 8000, in two ranges, 96 and 205, by global atomics 1030 and 288 000; with 86 000 in 16 ranges 514 and 1580.
 template <bool kLds, bool kQuads>
 __global__ void __launch_bounds__(kNeighbourThreads) balance_neighbours_kernel(int64_t N, int M, int K,
     const float* __restrict__ weights, const int64_t* __restrict__ indices, const uint8_t* __restrict__ rows,
     unsigned long long* __restrict__ sums, int* __restrict__ counts, BlockRows* __restrict__ blocks, unsigned* __restrict__ ticket) {
   extern __shared__ unsigned long long s_sums[];  // [M], then the counts [M]
   __shared__ int s_rows[2];
+  const int first = kLds ? blockIdx.y * kMostInLds : 0, in_range = kLds ? min(M - first, kMostInLds) : M;
   unsigned long long* sum = kLds ? s_sums : sums;
-  int* count = kLds ? (int*) (s_sums + M) : counts;
+  int* count = kLds ? (int*) (s_sums + in_range) : counts;
   if (kLds)
-    for (int c = threadIdx.x; c < M; c += kNeighbourThreads) sum[c] = 0, count[c] = 0;
+    for (int c = threadIdx.x; c < in_range; c += kNeighbourThreads) sum[c] = 0, count[c] = 0;
   if (threadIdx.x < 2) s_rows[threadIdx.x] = 0;
   __syncthreads();
   int counted = 0, invalid = 0;
@@ -514,19 +518,20 @@ __global__ void __launch_bounds__(kNeighbourThreads) balance_neighbours_kernel(i
           invalid = 1;
           continue;
         }
-        atomicAdd(&sum[(int) m[d]], (unsigned long long) __float2uint_rn(w[d] * kWeightUnits));
+        const unsigned at = (unsigned) ((int) m[d] - first);
+        if (at < (unsigned) in_range) atomicAdd(&sum[at], (unsigned long long) __float2uint_rn(w[d] * kWeightUnits));
         if (w[d] > best) best = w[d], where = (int) m[d];
       }
     }
-    if (best >= 0.0f) atomicAdd(&count[where], 1);
+    if (best >= 0.0f && (unsigned) (where - first) < (unsigned) in_range) atomicAdd(&count[where - first], 1);
   }
   if (counted) atomicAdd(&s_rows[0], counted);
   if (invalid) atomicOr(&s_rows[1], 1);
   __syncthreads();
   if (kLds)
-    for (int c = threadIdx.x; c < M; c += kNeighbourThreads)
-      sums[(size_t) blockIdx.x * M + c] = sum[c], counts[(size_t) blockIdx.x * M + c] = count[c];
-  if (threadIdx.x == 0) {
+    for (int c = threadIdx.x; c < in_range; c += kNeighbourThreads)
+      sums[(size_t) blockIdx.x * M + first + c] = sum[c], counts[(size_t) blockIdx.x * M + first + c] = count[c];
+  if (threadIdx.x == 0 && blockIdx.y == 0) {
     blocks[blockIdx.x] = BlockRows{s_rows[0], s_rows[1]};
     if (blockIdx.x == 0) *ticket = 0;
   }
@@ -688,10 +693,11 @@ int pass_blocks(int64_t N, int M, int dtype) {
   const int64_t most = std::min<int64_t>(kRowBlocks, std::max<int64_t>(32, ((int64_t) 1 << 25) / M));
   return (int) std::min(blocks, most);
 }
-bool in_lds(int64_t M) { return M <= kMostInLds; }
-int neighbour_blocks(int64_t N) {
+bool in_lds(int64_t M) { return M <= (int64_t) kMostRanges * kMostInLds; }
+int neighbour_blocks(int64_t N, int64_t M) {
   const int64_t blocks = (N + kNeighbourThreads - 1) / kNeighbourThreads;
-  return (int) (blocks < kNeighbourBlocks ? blocks : kNeighbourBlocks);
+  const int64_t ranges = in_lds(M) ? (M + kMostInLds - 1) / kMostInLds : 1;
+  return (int) std::min(blocks, kNeighbourBlocks / ranges);
 }
 
 // Logits that exceed the 256 MB memory-side cache are read past it.
@@ -815,7 +821,7 @@ FSGS_API int fsgs_balance_loss_backward(int64_t N, int M, int64_t ld, int dtype,
 
 FSGS_API size_t fsgs_neighbour_balance_workspace_bytes(int64_t N, int M) {
   if (N < 0 || M <= 0) return 0;
-  const int G = neighbour_blocks(N);
+  const int G = neighbour_blocks(N, M);
   return Workspace(in_lds(M) ? G : 1, M, 8, G).bytes;
 }
 
@@ -825,7 +831,7 @@ FSGS_API int fsgs_neighbour_balance_forward(int64_t N, int M, int K, const float
   FSGS_REQUIRE(N >= 0 && N < (int64_t) 0x7fffffff && M > 0 && K >= 1, "%s: bad arguments", what);
   FSGS_REQUIRE((N == 0 || (weights && indices)) && loss && counts && importance && totals && workspace, "%s: null pointer", what);
   FSGS_REQUIRE((uintptr_t) weights % 4 == 0 && (uintptr_t) indices % 8 == 0 && (uintptr_t) workspace % 8 == 0, "%s: misaligned address", what);
-  const int G = neighbour_blocks(N), G_sums = in_lds(M) ? G : 1;
+  const int G = neighbour_blocks(N, M), G_sums = in_lds(M) ? G : 1;
   const Workspace ws(G_sums, M, 8, G);
   if (workspace_bytes < ws.bytes) return fsgs::fail(kWorkspaceSmall, "%s: the workspace is too small", what);
   char* at = (char*) workspace;
@@ -841,8 +847,9 @@ FSGS_API int fsgs_neighbour_balance_forward(int64_t N, int M, int K, const float
     const bool quads = K % 4 == 0 && ((uintptr_t) weights | (uintptr_t) indices) % 16 == 0;
     auto kernel = in_lds(M) ? (quads ? balance_neighbours_kernel<true, true> : balance_neighbours_kernel<true, false>)
                             : (quads ? balance_neighbours_kernel<false, true> : balance_neighbours_kernel<false, false>);
-    hipLaunchKernelGGL(kernel, dim3(G), dim3(kNeighbourThreads), in_lds(M) ? (size_t) M * 12 : 0, s, N, M, K, weights, indices, rows, sums,
-                       block_counts, blocks, ticket);
+    const dim3 grid(G, in_lds(M) ? div_up(M, kMostInLds) : 1);
+    hipLaunchKernelGGL(kernel, grid, dim3(kNeighbourThreads), in_lds(M) ? (size_t) std::min(M, kMostInLds) * 12 : 0, s, N, M, K, weights,
+                       indices, rows, sums, block_counts, blocks, ticket);
   }
   if (const int rc = check_launch(what)) return rc;
   hipLaunchKernelGGL(balance_totals_kernel<unsigned long long>, dim3(div_up(M, kTotalColumns)), dim3(1024), 0, s, G_sums, G, M, sums, block_counts,

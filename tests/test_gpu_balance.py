@@ -275,9 +275,15 @@ def test_neighbour_balance(device, N, M, K):
         assert (abs(npy(grad).astype(np.float64) - want) <= bound).all()
 
 
+@pytest.mark.parametrize('N,M,K', [(300, 10_800, 3), (300, 10_801, 4), (700, 86_400, 3), (700, 86_401, 4), (20_000, 30_000, 2)])
+def test_neighbour_balance_of_many_superpoints(device, N, M, K):
+    """Several ranges of superpoints, and more than there are ranges for."""
+    test_neighbour_balance(device, N, M, K)
+
+
 def test_bad_weights_and_indices_show(device):
     from fast_sp_gs_amd.balance import neighbour_balance
-    for M in (50, 6000):
+    for M in (50, 6000, 90_000):
         for bad_w, bad_i in ((float('nan'), 3), (-0.1, 3), (1.5, 3), (float('inf'), 3), (0.5, -1), (0.5, M), (0.5, 1 << 40)):
             w = torch.full((2000, 3), 1 / 3, device=device)
             index = torch.randint(0, M, (2000, 3), device=device)
