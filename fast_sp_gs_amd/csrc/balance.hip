@@ -28,7 +28,7 @@ constexpr int kMostChoices   = 64;
 constexpr int kRowBlocks     = 768;   // of the pass over logits
 // Threads of its blocks, and wavefronts that share a SIMD's registers: with 64 values in each lane one has them to itself.
 constexpr int row_threads(int vals) { return vals >= 32 ? 256 : 512; }
-constexpr int row_waves(int vals, bool narrow) { return vals == 64 ? 1 : vals == 32 ? (narrow ? 3 : 2) : vals == 16 ? 3 : 4; }
+constexpr int row_waves(int vals) { return vals == 64 ? 1 : vals >= 16 ? 3 : 4; }
 constexpr int kMostInLanes   = 4096;  // superpoints whose row is held by the lanes of one wavefront
 constexpr int kNeighbourBlocks = 256;
 constexpr int kNeighbourThreads = 1024;
@@ -161,15 +161,24 @@ __device__ __forceinline__ int reaching(const float x[kVals], float t) {
 // Counts the row's K largest values above -inf, the lowest column first among equals. `lane_top`: the largest of the lane, `top` of the row,
 // ordered. The K-th largest of the lanes' own largest is reached by at least K values, and mostly by no other: 4 of 512 values lie
 // in 4 of 64 lanes in 9 rows of 10. Otherwise the threshold rises value by value, after a walk down from the top where that is nearer.
-// What is chosen among values equal to the threshold is counted in LDS.
+// What is chosen among values equal to the threshold is counted in LDS, the rest in registers against the next value above it. The number of
+// values above the threshold is taken first and the next value sought only where it has to rise (100 000 x 2000, 8 chosen: 214 -> 173 us).
 template <typename T, int kLanes, int kVals>
 __device__ __forceinline__ void choose(const float x[kVals], int lane_top, int top, int K, int lane, int count[kVals], int* s_count) {
   const int lowest = ordered(-INFINITY);
   int t_ordered = top;
   for (int r = 1; r < K; ++r) t_ordered = row_max<kLanes>(lane_top < t_ordered ? lane_top : lowest);
   float t = unordered(max(t_ordered, ordered(kLowest)));
-  int n = reaching<kLanes, kVals>(x, t);
+  int n = 0;
+  bool hit[kVals];
+#pragma unroll
+  for (int j = 0; j < kVals; ++j) hit[j] = x[j] >= t, n += kLanes == 64 ? (int) __popcll(wave_ballot(hit[j])) : hit[j] ? 1 : 0;
+  if (kLanes != 64) n = row_count<kLanes>(n);
+#pragma unroll
+  for (int j = 0; j < kVals; ++j) count[j] += hit[j] ? 1 : 0;
   if (wave_ballot(n > K)) {
+#pragma unroll
+    for (int j = 0; j < kVals; ++j) count[j] -= hit[j] ? 1 : 0;
     if (wave_ballot(n > 2 * K)) {
       float s = unordered(top);
       for (int r = 1; r < K; ++r) {
@@ -182,22 +191,42 @@ __device__ __forceinline__ void choose(const float x[kVals], int lane_top, int t
       const int m = reaching<kLanes, kVals>(x, s);
       if (n > 2 * K) t = s, n = m;
     }
-    bool ties = false;  // more than K reach t, fewer than K what is above it
-    int left = 0;       // of those equal to t
-    float all_from = t;
-    while (wave_ballot(n > K && !ties)) {
+    int left = -1;  // of the values equal to t, once fewer than K lie above it
+    while (wave_ballot(n > K && left < 0)) {
+      int greater = 0;
+#pragma unroll
+      for (int j = 0; j < kVals; ++j) greater += kLanes == 64 ? (int) __popcll(wave_ballot(x[j] > t)) : x[j] > t ? 1 : 0;
+      if (kLanes != 64) greater = row_count<kLanes>(greater);
+      const bool higher = n > K && greater >= K;
+      if (n > K && !higher) left = K - greater;
+      if (!wave_ballot(higher)) continue;
       float above = INFINITY;
 #pragma unroll
       for (int j = 0; j < kVals; ++j) above = fminf(above, x[j] > t ? x[j] : INFINITY);
       above = unordered(row_min<kLanes>(ordered(above)));
-      const int m = above > t ? reaching<kLanes, kVals>(x, above) : 0;
-      if (n > K && !ties) {
-        if (m >= K) t = all_from = above, n = m;
-        else ties = true, left = K - m, all_from = m > 0 ? above : __builtin_nanf("");  // nothing reaches a NaN
-      }
+      if (higher) t = above, n = greater;
     }
-    int at = -1;
-    while (wave_ballot(left > 0)) {
+    if (kLanes == 64 && left > 0) {
+      // columns rise with the piece, the lane, the value of the piece: over the comparisons' lane masks
+      constexpr int kPiece = 16 / sizeof(T);
+#pragma unroll
+      for (int i = 0; i < kVals; i += kPiece) {
+        unsigned long long equal[kPiece], any = 0;
+#pragma unroll
+        for (int k = 0; k < kPiece; ++k) equal[k] = wave_ballot(x[i + k] == t), any |= equal[k];
+        for (; any && left > 0; any &= any - 1) {
+          const int l = __builtin_ctzll(any);
+#pragma unroll
+          for (int k = 0; k < kPiece; ++k)
+            if (((equal[k] >> l) & 1) && left > 0) {
+              if (lane == 0) atomicAdd(&s_count[column<T, kLanes>(l, i + k)], 1);
+              --left;
+            }
+        }
+      }
+      left = 0;
+    }
+    for (int at = -1, more = left; kLanes < 64 && wave_ballot(more > 0); --more) {
       const int l = keep_local(lane);  // or every column's index stays in a register of its own
       int where = 0x7fffffff;
 #pragma unroll
@@ -206,17 +235,31 @@ __device__ __forceinline__ void choose(const float x[kVals], int lane_top, int t
         where = min(where, x[j] == t && c > at ? c : 0x7fffffff);
       }
       at = row_min<kLanes>(where);
-      if (left > 0 && lane == 0) atomicAdd(&s_count[at], 1);
-      --left;
+      if (more > 0 && lane == 0) atomicAdd(&s_count[at], 1);
     }
-    t = ties ? all_from : t;
-  }
+    // those above it, above 0 where it is -0; what follows an infinity is a NaN, which nothing reaches
+    if (left >= 0) t = unordered(ordered(t + 0.0f) + 1);
 #pragma unroll
-  for (int j = 0; j < kVals; ++j) count[j] += x[j] >= t ? 1 : 0;
+    for (int j = 0; j < kVals; ++j) count[j] += x[j] >= t ? 1 : 0;
+  }
+}
+
+// exp(x - shift) of the row's values. The shift's product with log2 e is rounded once for the whole row, a factor that the row's sum has too:
+// one multiply-add a value. Where the product could overflow the difference is taken first.
+template <int kVals>
+__device__ __forceinline__ void exponentials(float x[kVals], float shift) {
+  const bool far = fabsf(shift) > 1e38f;
+  if (wave_ballot(far)) {
+#pragma unroll
+    for (int j = 0; j < kVals; ++j) x[j] = far ? x[j] - shift : x[j];
+  }
+  const float s = far ? 0.0f : shift * kLog2e;
+#pragma unroll
+  for (int j = 0; j < kVals; ++j) x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], kLog2e, -s));
 }
 
 template <typename T, int kLanes, int kVals, Access kAccess>
-__global__ void __launch_bounds__(row_threads(kVals), row_waves(kVals, sizeof(T) == 2 && kAccess != kSingle)) balance_rows_kernel(int64_t N, int M, int64_t ld, int K,
+__global__ void __launch_bounds__(row_threads(kVals), row_waves(kVals)) balance_rows_kernel(int64_t N, int M, int64_t ld, int K,
     const T* __restrict__ logits, const uint8_t* __restrict__ rows, float2* __restrict__ stats, float* __restrict__ sums,
     int* __restrict__ counts, BlockRows* __restrict__ blocks, unsigned* __restrict__ ticket) {
   constexpr int kRows = 64 / kLanes, kThreads = row_threads(kVals), kWaves = kThreads / 64;
@@ -250,8 +293,9 @@ __global__ void __launch_bounds__(row_threads(kVals), row_waves(kVals, sizeof(T)
     // a row without a number (top is -inf): the sum is 0, or NaN where one of its values is, which counts
     const float top = unordered(top_ordered), shift = top == -INFINITY ? 0.0f : top;
     float total = 0.0f;
+    exponentials<kVals>(x, shift);
 #pragma unroll
-    for (int j = 0; j < kVals; ++j) x[j] = __builtin_amdgcn_exp2f((x[j] - shift) * kLog2e), total += x[j];
+    for (int j = 0; j < kVals; ++j) total += x[j];
     total = row_sum<kLanes>(total);
     const bool counts_in = !(total == 0.0f);
     const float scale = counts_in ? __builtin_amdgcn_rcpf(total) : 0.0f;
@@ -333,11 +377,9 @@ __global__ void __launch_bounds__(256) balance_rows_backward_kernel(int64_t N, i
     const bool on = on_of(at, stat);
     float x[kVals], mean = 0.0f;
     row.template values<kAccess>(x, M, full, on, lane);
+    exponentials<kVals>(x, stat.x);
 #pragma unroll
-    for (int j = 0; j < kVals; ++j) {
-      x[j] = __builtin_amdgcn_exp2f((x[j] - stat.x) * kLog2e) * stat.y;
-      mean = fmaf(x[j], slope[j], mean);
-    }
+    for (int j = 0; j < kVals; ++j) x[j] *= stat.y, mean = fmaf(x[j], slope[j], mean);
     mean = row_sum<kLanes>(mean);
     if (at >= N) return;
     T* out = grad + at * M;
