@@ -21,12 +21,13 @@ def balance_loss(logits: Tensor, K: int = 1, rows: Optional[Tensor] = None) -> T
     """(loss [], counts [M] int32, importance P [M]) of association logits [N, M] (float32, float16 or bfloat16; sums in float32 or more),
     whose softmax over the superpoints is the weight. Equal logits are chosen by the lowest index; -inf marks a superpoint that a point
     may not use, and is never chosen. `rows` [N] bool: the points that count; the others' logits are not looked at and get a gradient
-    of 0, as do points whose logits are all -inf. K is at most 64. loss and importance are differentiable in the logits."""
+    of 0, as do points whose logits are all -inf. K is at most 64, M below 2^26, N below 2^31. loss and importance are differentiable in the
+    logits."""
     return host.balance_loss(logits, K, rows)
 
 
 def neighbour_balance(weights: Tensor, indices: Tensor, M: int, rows: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
     """`balance_loss` of neighbour weights [N, K] in [0, 1] with their superpoints' indices [N, K] (what `calc_LBS_weight` returns), of
     M superpoints; chosen is a point's neighbour of largest weight, the first of equal ones. An index may be there twice. A weight outside
-    [0, 1] or an index outside [0, M) in a row that counts makes loss and importance NaN. Weights are added in units of 2^-31."""
+    [0, 1] or an index outside [0, M) in a row that counts makes loss and importance NaN. Weights are added in units of 2^-31; N K is below 2^33."""
     return host.neighbour_balance(weights, indices, M, rows)

@@ -467,7 +467,7 @@ bool streams(int n, const int64_t* count, size_t bytes_an_element) {
    : (dtype) == kFloat16 ? ((stream) ? kernel<__half, true> : kernel<__half, false>)                 \
                          : ((stream) ? kernel<__hip_bfloat16, true> : kernel<__hip_bfloat16, false>))
 
-// first[q]: blocks before tensor q at `per_block` elements a block
+// first[q]: blocks before tensor q at `per_block` elements a block. A launch has 2^32 threads at most, in blocks of 256.
 template <typename Table>
 int lay_out(const char* what, Table& t, unsigned* first, int n, const int64_t* count, int64_t per_block) {
   int64_t blocks = 0;
@@ -475,7 +475,7 @@ int lay_out(const char* what, Table& t, unsigned* first, int n, const int64_t* c
     FSGS_REQUIRE(count[q] >= 0, "%s: bad tensor %d", what, q);
     t.count[q] = count[q], first[q] = (unsigned) blocks;
     blocks += (count[q] + per_block - 1) / per_block;
-    FSGS_REQUIRE(blocks < (int64_t) 0x7fffffff, "%s: too many elements", what);
+    FSGS_REQUIRE(blocks < (int64_t) 1 << 24, "%s: more than %lld elements in a launch", what, (long long) (per_block << 24));
   }
   first[n] = (unsigned) blocks;
   t.n = n;

@@ -799,6 +799,11 @@ void launch_rows_backward(int G, int64_t N, int M, int64_t ld, const void* logit
 }
 #undef FSGS_ROW_KERNELS
 
+// The totals' launch has 1024 threads for 16 superpoints, 2^32 of them at most.
+constexpr int kMostSuperpoints = (1 << 26) - 1;
+// Sums of weights have 64 bits, 31 of them below the point.
+constexpr int64_t kMostPairs = ((int64_t) 1 << 33) - 1;
+
 bool is_type(int type) { return type == FSGS_DTYPE_F32 || type == FSGS_DTYPE_F16 || type == FSGS_DTYPE_BF16; }
 
 }  // namespace
@@ -819,6 +824,7 @@ FSGS_API int fsgs_balance_loss_forward(int64_t N, int M, int64_t ld, int K, int 
     void* stream) {
   const char* what = "balance_loss";
   FSGS_REQUIRE(N >= 0 && N < (int64_t) 0x7fffffff && M > 0 && is_type(dtype) && (N <= 1 || ld >= M), "%s: bad arguments", what);
+  FSGS_REQUIRE(M <= kMostSuperpoints, "%s: more than %d superpoints", what, kMostSuperpoints);
   FSGS_REQUIRE(K >= 1 && K <= M && K <= kMostChoices, "%s: K must be in [1, min(M, %d)]", what, kMostChoices);
   FSGS_REQUIRE((N == 0 || logits) && loss && counts && importance && totals && workspace, "%s: null pointer", what);
   FSGS_REQUIRE((uintptr_t) logits % (dtype == FSGS_DTYPE_F32 ? 4 : 2) == 0 && (uintptr_t) stats % 8 == 0 && (uintptr_t) workspace % 8 == 0,
@@ -871,6 +877,8 @@ FSGS_API int fsgs_neighbour_balance_forward(int64_t N, int M, int K, const float
     float* loss, int32_t* counts, float* importance, int64_t* totals, void* workspace, size_t workspace_bytes, void* stream) {
   const char* what = "neighbour_balance";
   FSGS_REQUIRE(N >= 0 && N < (int64_t) 0x7fffffff && M > 0 && K >= 1, "%s: bad arguments", what);
+  FSGS_REQUIRE(M <= kMostSuperpoints, "%s: more than %d superpoints", what, kMostSuperpoints);
+  FSGS_REQUIRE(N * K <= kMostPairs, "%s: more than %lld pairs of points and neighbours", what, (long long) kMostPairs);
   FSGS_REQUIRE((N == 0 || (weights && indices)) && loss && counts && importance && totals && workspace, "%s: null pointer", what);
   FSGS_REQUIRE((uintptr_t) weights % 4 == 0 && (uintptr_t) indices % 8 == 0 && (uintptr_t) workspace % 8 == 0, "%s: misaligned address", what);
   const int G = neighbour_blocks(N, M), G_sums = in_lds(M) ? G : 1;

@@ -88,6 +88,7 @@ struct Call {
     if (n == 0) return;
     const at::Device device = params[0].device();
     device_steps = steps[0].is_cuda();
+    int64_t elements = 0;
     for (size_t k = 0; k < n; ++k) {
       const Tensor &p = params[k], &g = given[k];
       require_device(w, "param", p, device), require_device(w, "grad", g, device);
@@ -96,6 +97,8 @@ struct Call {
       if (g.sizes() != p.sizes()) fail(w + ": tensor " + number(k) + "'s gradient differs from it in shape");
       if (g.scalar_type() != p.scalar_type())
         fail(w + ": tensor " + number(k) + "'s gradient must have dtype " + dtype_text(p.scalar_type()) + ", got " + dtype_text(g.scalar_type()));
+      elements += p.numel() + 1024;  // the last block of a tensor is not always a whole one
+      if (elements >= (int64_t) 1 << 34) fail(w + ": more elements than a launch takes (2^34)");
       const Tensor& s = steps[k];
       if (!s.defined() || s.numel() != 1) fail(w + ": a step count is one number");
       if (s.is_cuda() != device_steps) fail(w + ": step counts must all be on the host or all on the device");

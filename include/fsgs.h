@@ -992,7 +992,7 @@ int fsgs_adam_masked_update_multi(int n_tensors, int64_t N, const int64_t* M, co
  * one that is being taken), lr, eps, decay and the addresses. dtype (FSGS_DTYPE_F32, _F16, _BF16) is that of param and grad; m and v are
  * float32. norm_and_factor (device, optional): what fsgs_grad_norm_factor wrote, c = norm_and_factor[1]; 1 without it.
  * rates (device, optional): what fsgs_adamw_rates wrote for the same tensors; step may be NULL then. Addresses need the alignment of
- * their element type; those of four elements are moved in one access. */
+ * their element type; those of four elements are moved in one access. A launch takes fewer than 2^34 elements. */
 int fsgs_adamw_max_tensors(void);
 int fsgs_adamw_update_multi(int n_tensors, int dtype, const int64_t* count, const double* step, const double* lr, double b1,
     double b2, const double* eps, const double* decay, const void* rates, const float* norm_and_factor, void* const* param,
@@ -1028,7 +1028,7 @@ int fsgs_grad_norm_factor(int n_sums, const double* sums, double max_norm, float
  * logits above -inf, the lowest index first (K <= fsgs_balance_max_choices()). rows[N] (optional): 0 leaves a row out, unread. stats[N][2]
  * (optional, 8-byte aligned): what the backward needs of each row. workspace: fsgs_balance_loss_workspace_bytes bytes, 8-byte aligned.
  * The backward writes grad[N, M] (dtype, contiguous) = p (a - sum p a), a = (g_loss M f + g_importance) / T; either of the two upstream
- * gradients (device, g_loss one float, g_importance[M]) may be NULL. N < 2^31. */
+ * gradients (device, g_loss one float, g_importance[M]) may be NULL. N < 2^31, M < 2^26. */
 int fsgs_balance_max_choices(void);
 size_t fsgs_balance_loss_workspace_bytes(int64_t N, int M, int dtype);
 int fsgs_balance_loss_forward(int64_t N, int M, int64_t ld, int K, int dtype, const void* logits, const uint8_t* rows,
@@ -1037,7 +1037,7 @@ int fsgs_balance_loss_forward(int64_t N, int M, int64_t ld, int K, int dtype, co
 int fsgs_balance_loss_backward(int64_t N, int M, int64_t ld, int dtype, const void* logits, const float* stats,
     const int32_t* counts, const int64_t* totals, const float* g_loss, const float* g_importance, void* grad, void* stream);
 /* The same of weights[N, K] in [0, 1] with indices[N, K] in [0, M): a row chooses its largest weight, the first of equal ones. A weight or
- * an index outside, in a row that counts, makes loss and importance NaN. The backward's grad[N, K] = a[index], 0 in rows left out. */
+ * an index outside, in a row that counts, makes loss and importance NaN. The backward's grad[N, K] = a[index], 0 in rows left out. N K < 2^33. */
 size_t fsgs_neighbour_balance_workspace_bytes(int64_t N, int M);
 int fsgs_neighbour_balance_forward(int64_t N, int M, int K, const float* weights, const int64_t* indices, const uint8_t* rows,
     float* loss, int32_t* counts, float* importance, int64_t* totals, void* workspace, size_t workspace_bytes, void* stream);

@@ -70,6 +70,21 @@ def test_c_entries_refuse_without_touching_the_gpu():
     assert L.fsgs_adamw8_pack_multi(1, A(count), A(odd), A(odd), A(odd), None) != 0
 
 
+def test_more_than_a_launch_holds_is_refused():
+    import ctypes
+    from fast_sp_gs_amd import lib
+    L = lib.load()
+    A = ctypes.addressof
+    one, at = (ctypes.c_double * 1)(1.0), (ctypes.c_void_p * 1)(4097)  # an address that is no float's
+    many = (ctypes.c_int64 * 1)(1 << 34)  # 2^24 blocks of 1024 elements, 256 threads each
+    assert L.fsgs_adamw_update_multi(1, 0, A(many), A(one), A(one), 0.9, 0.999, A(one), A(one), None, None, A(at), A(at), A(at), A(at), None) != 0
+    assert b'elements' in L.fsgs_last_error()
+    assert L.fsgs_adamw8_update_multi(1, 0, A(many), A(one), A(one), 0.9, 0.999, A(one), A(one), 0, None, None, A(at), A(at), A(at), None) != 0
+    assert b'elements' in L.fsgs_last_error()
+    assert L.fsgs_adamw8_unpack_multi(1, 0, A(many), A(at), A(at), A(at), None) != 0 and b'elements' in L.fsgs_last_error()
+    assert L.fsgs_adamw8_pack_multi(1, A(many), A(at), A(at), A(at), None) != 0 and b'elements' in L.fsgs_last_error()
+
+
 def test_the_roundings_noise_is_even():
     """The hash's two halves over elements, steps and seeds: means, variances and correlations of uniform numbers (five sigma)."""
     n = 1 << 18

@@ -39,3 +39,16 @@ def test_c_entries_refuse_without_touching_the_gpu():
     for wrong in (dict(N=-1), dict(i=None), dict(g=None), dict(grad=None), dict(grad=A + 2), dict(i=A + 4)):
         assert near_back(**wrong) != 0, wrong
     assert near_back(N=0) == 0
+
+
+def test_what_sums_and_launches_cannot_hold():
+    from fast_sp_gs_amd import lib
+    L = lib.load()
+    A, big = 4096, 1 << 60
+    assert L.fsgs_balance_loss_forward(4, 1 << 26, 1 << 26, 1, 0, A, None, A, A, A, A, A, A, big, None) != 0
+    assert b'superpoints' in L.fsgs_last_error()
+    assert L.fsgs_neighbour_balance_forward(4, 1 << 26, 3, A, A, None, A, A, A, A, A, big, None) != 0
+    assert b'superpoints' in L.fsgs_last_error()
+    # 2^33 weights of 1 at one superpoint, in units of 2^-31, are 2^64
+    assert L.fsgs_neighbour_balance_forward(1 << 30, 70, 8, A, A, None, A, A, A, A, A, big, None) != 0
+    assert b'pairs' in L.fsgs_last_error()

@@ -508,3 +508,13 @@ def test_wrong_tensors_are_refused(device):
     theirs = torch.optim.AdamW([torch.nn.Parameter(ok())], amsgrad=True)
     with pytest.raises(ValueError, match='amsgrad'):
         AdamW([torch.nn.Parameter(ok())]).load_state_dict(theirs.state_dict())
+
+
+def test_more_elements_than_a_launch_takes_are_refused(device):
+    from fast_sp_gs_amd.adamw import adamw8_step
+    n = 1 << 34  # nothing of it is touched
+    p = torch.empty(n, dtype=torch.bfloat16, device=device)
+    step, state = torch.zeros(()), torch.empty(n // 256 * 514, dtype=torch.uint8, device=device)
+    with pytest.raises(RuntimeError, match='elements'):
+        adamw8_step([p], [p], [state], [step])
+    assert float(step) == 0.0
