@@ -1,6 +1,7 @@
 #include "balance.hpp"
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 
 #include <climits>
 
@@ -32,6 +33,17 @@ void require_rows(const char* what, const Tensor& rows, const Tensor& like) {
   if (!rows.defined()) return;
   require(what, "rows", rows, at::kBool), require_shape(what, "rows", rows, {like.size(0)});
   if (rows.device() != like.device()) fail(std::string(what) + ": all tensors of a call must be on one device");
+}
+
+// A captured backward of a leaf whose accumulation node an eager graph on the default stream keeps alive would have that stream wait for
+// the capture, which ends it and the process: refused while nothing is recorded.
+void refuse_capture_beside_eager(const char* what, const char* name, const Tensor& t) {
+  if (!t.is_leaf() || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!node) return;
+  const auto stream = node->stream();
+  if (stream && stream->id() == 0)
+    fail(std::string(what) + ": " + name + " is part of an eager graph that is still alive: drop that graph before this call is captured");
 }
 
 OptTensor given(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
@@ -149,6 +161,7 @@ std::tuple<Tensor, Tensor, Tensor> balance_loss(const Tensor& logits, int64_t K,
   const c10::DeviceGuard guard(logits.device());
   const Tensor x = rows_of(logits);
   if (at::GradMode::is_enabled() && x.requires_grad()) {
+    refuse_capture_beside_eager(what, "logits", logits);
     const variable_list out = RowsNode::apply(x, K, given(on));
     return {out[0], out[1], out[2]};
   }
@@ -168,6 +181,7 @@ std::tuple<Tensor, Tensor, Tensor> neighbour_balance(const Tensor& weights, cons
   if (M < 1 || M > INT_MAX) fail("neighbour_balance: M must be positive");
   const c10::DeviceGuard guard(w.device());
   if (at::GradMode::is_enabled() && w.requires_grad()) {
+    refuse_capture_beside_eager(what, "weights", weights);
     const variable_list out = NeighboursNode::apply(w, index, M, given(on));
     return {out[0], out[1], out[2]};
   }

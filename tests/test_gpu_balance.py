@@ -337,6 +337,29 @@ def test_captured_and_on_another_stream(device):
         assert all(torch.equal(a, b) for a, b in zip(eager(k), want[k]))
 
 
+def test_captured_beside_an_eager_graph_of_the_same_leaves(device):
+    """The default stream, on which the eager graph accumulates, cannot join a capture: refused before anything is recorded."""
+    from fast_sp_gs_amd.balance import balance_loss, neighbour_balance
+    x = torch.randn(300, 20, device=device, requires_grad=True)
+    w = torch.full((300, 2), 0.5, device=device, requires_grad=True)
+    index = torch.randint(0, 20, (300, 2), device=device)
+    calls = [lambda: balance_loss(x)[0], lambda: neighbour_balance(w, index, 20)[0]]
+    for leaf, call in zip((x, w), calls):
+        alive = call()
+        want, = torch.autograd.grad(alive, leaf, retain_graph=True)
+        with pytest.raises(RuntimeError, match='eager graph'):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+        del alive
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got, = torch.autograd.grad(call(), leaf)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+
+
 def test_differentiated_once(device):
     from fast_sp_gs_amd.balance import balance_loss
     x = torch.randn(6, 5, device=device, requires_grad=True)
