@@ -17,6 +17,7 @@
 #include <hip/hip_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/fsgs.h"
 #include "common.hpp"
@@ -64,33 +65,34 @@ template <int kCtrl>
 __device__ __forceinline__ int moved(int x) {
   return __builtin_amdgcn_update_dpp(0, x, kCtrl, 0xf, 0xf, true);
 }
+// `none`: what f leaves its other argument as it is with
 template <int kLanes, typename F>
-__device__ __forceinline__ int over_lanes(int x, F f) {
+__device__ __forceinline__ int over_lanes(int x, int none, F f) {
   x = f(x, moved<0xB1>(x)), x = f(x, moved<0x4E>(x));  // quad_perm: neighbours, then pairs of them
   if (kLanes >= 8) x = f(x, moved<0x141>(x));          // row_half_mirror
   if (kLanes >= 16) x = f(x, moved<0x140>(x));         // row_mirror
   if (kLanes == 64) {
-    const int a = f(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16));
-    const int b = f(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48));
-    x = f(a, b);
+    x = f(x, __builtin_amdgcn_update_dpp(none, x, 0x142, 0xa, 0xf, false));  // row_bcast15: of 16 lanes to the next 16
+    x = f(x, __builtin_amdgcn_update_dpp(none, x, 0x143, 0xc, 0xf, false));  // row_bcast31: of 32 to the next
+    x = __builtin_amdgcn_readlane(x, 63);
   }
   return x;
 }
 template <int kLanes>
 __device__ __forceinline__ int row_max(int x) {
-  return over_lanes<kLanes>(x, [](int a, int b) { return max(a, b); });
+  return over_lanes<kLanes>(x, (int) 0x80000000, [](int a, int b) { return max(a, b); });
 }
 template <int kLanes>
 __device__ __forceinline__ int row_min(int x) {
-  return over_lanes<kLanes>(x, [](int a, int b) { return min(a, b); });
+  return over_lanes<kLanes>(x, 0x7fffffff, [](int a, int b) { return min(a, b); });
 }
 template <int kLanes>
 __device__ __forceinline__ int row_count(int x) {
-  return over_lanes<kLanes>(x, [](int a, int b) { return a + b; });
+  return over_lanes<kLanes>(x, 0, [](int a, int b) { return a + b; });
 }
 template <int kLanes>
 __device__ __forceinline__ float row_sum(float x) {
-  return as_float(over_lanes<kLanes>((int) as_uint(x), [](int a, int b) { return (int) as_uint(as_float(a) + as_float(b)); }));
+  return as_float(over_lanes<kLanes>((int) as_uint(x), 0, [](int a, int b) { return (int) as_uint(as_float(a) + as_float(b)); }));
 }
 // Floats as integers of the same order (-0 directly below 0): their maximum takes one instruction with a lane's exchange, where that
 // of floats quiets its operands first. It is its own inverse.
@@ -108,12 +110,27 @@ __device__ __forceinline__ int column(int lane, int j) {
 // How logits are read: element by element; in pieces, which are aligned and end where the row ends; in pieces past the caches.
 enum Access { kSingle, kWhole, kStream };
 
+// Element j of words as they lie in memory.
+template <typename T>
+__device__ __forceinline__ float element(const uint32_t* word, int j);
+template <>
+__device__ __forceinline__ float element<float>(const uint32_t* word, int j) { return as_float(word[j]); }
+template <>
+__device__ __forceinline__ float element<__hip_bfloat16>(const uint32_t* word, int j) {
+  return as_float(j & 1 ? word[j / 2] & 0xffff0000u : word[j / 2] << 16);
+}
+template <>
+__device__ __forceinline__ float element<__half>(const uint32_t* word, int j) {
+  return (float) __builtin_bit_cast(_Float16, (uint16_t) (word[j / 2] >> (j & 1) * 16));
+}
+
 // A lane's part of a row as it lies in memory. A row that is not `on` is read where the first one is, a column that there is not where the
-// row begins: no branch stands between the loads, so that they stay in flight while the row before is worked on.
+// row begins: no branch stands between the loads, so that they stay in flight while the row before is worked on. It is kept in words: the
+// compiler would take elements of 16 bits apart as they arrive and put them into place again.
 template <typename T, int kLanes, int kVals>
 struct Row {
   static constexpr int kPiece = 16 / sizeof(T);
-  Pack<T, kPiece> piece[kVals / kPiece];
+  uint32_t word[kVals * sizeof(T) / 4];
 
   template <Access kAccess>
   __device__ __forceinline__ void load(const T* __restrict__ row, int M, int lane) {
@@ -121,19 +138,26 @@ struct Row {
     for (int i = 0; i < kVals / kPiece; ++i) {
       const int c = column<T, kLanes>(lane, i * kPiece);
       typedef uint32_t Raw __attribute__((ext_vector_type(4)));
-      if (kAccess == kStream)
-        piece[i] = __builtin_bit_cast(Pack<T, kPiece>, __builtin_nontemporal_load((const Raw*) (row + (c < M ? c : 0))));
-      else if (kAccess == kWhole) piece[i] = *(const Pack<T, kPiece>*) (row + (c < M ? c : 0));
-      else
+      Raw q;
+      if (kAccess == kSingle) {
+        typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type x[kPiece];
 #pragma unroll
-        for (int k = 0; k < kPiece; ++k) piece[i].x[k] = row[c + k < M ? c + k : 0];
+        for (int k = 0; k < kPiece; ++k) __builtin_memcpy(&x[k], row + (c + k < M ? c + k : 0), sizeof(T));
+        q = __builtin_bit_cast(Raw, x);
+      } else if (kAccess == kWhole) {
+        q = *(const Raw*) (row + (c < M ? c : 0));
+      } else {
+        q = __builtin_nontemporal_load((const Raw*) (row + (c < M ? c : 0)));
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) word[4 * i + k] = q[k];
     }
   }
   // -inf for what there is not; `full`: every lane has kVals columns
   template <Access kAccess>
   __device__ __forceinline__ void values(float x[kVals], int M, bool full, bool on, int lane) const {
 #pragma unroll
-    for (int j = 0; j < kVals; ++j) x[j] = to_float(piece[j / kPiece].x[j % kPiece]);
+    for (int j = 0; j < kVals; ++j) x[j] = element<T>(word, j);
     if (wave_ballot(!on)) {
 #pragma unroll
       for (int j = 0; j < kVals; ++j) x[j] = on ? x[j] : -INFINITY;
@@ -149,20 +173,12 @@ struct Row {
   }
 };
 
-// How many values of the row reach t. A row that has the wavefront to itself is counted by the comparisons' lane masks.
-template <int kLanes, int kVals>
-__device__ __forceinline__ int reaching(const float x[kVals], float t) {
-  int n = 0;
-#pragma unroll
-  for (int j = 0; j < kVals; ++j) n += kLanes == 64 ? (int) __popcll(wave_ballot(x[j] >= t)) : x[j] >= t ? 1 : 0;
-  return kLanes == 64 ? n : row_count<kLanes>(n);
-}
-
 // Counts the row's K largest values above -inf, the lowest column first among equals. `lane_top`: the largest of the lane, `top` of the row,
 // ordered. The K-th largest of the lanes' own largest is reached by at least K values, and mostly by no other: 4 of 512 values lie
-// in 4 of 64 lanes in 9 rows of 10. Otherwise the threshold rises value by value, after a walk down from the top where that is nearer.
-// What is chosen among values equal to the threshold is counted in LDS, the rest in registers against the next value above it. The number of
-// values above the threshold is taken first and the next value sought only where it has to rise (100 000 x 2000, 8 chosen: 214 -> 173 us).
+// in 4 of 64 lanes in 9 rows of 10. What reaches it is counted at once, in the columns' registers (a row that has the wavefront to itself is
+// counted by the comparisons' lane masks). Where there are more, those equal to the threshold are taken back and the threshold rises to the
+// next value, until K are left or fewer; then the first of the last ones taken back are counted after all, in LDS. Where the K-th value is
+// nearer to the top than to the threshold, a walk down from the top comes first.
 template <typename T, int kLanes, int kVals>
 __device__ __forceinline__ void choose(const float x[kVals], int lane_top, int top, int K, int lane, int count[kVals], int* s_count) {
   const int lowest = ordered(-INFINITY);
@@ -170,77 +186,88 @@ __device__ __forceinline__ void choose(const float x[kVals], int lane_top, int t
   for (int r = 1; r < K; ++r) t_ordered = row_max<kLanes>(lane_top < t_ordered ? lane_top : lowest);
   float t = unordered(max(t_ordered, ordered(kLowest)));
   int n = 0;
-  bool hit[kVals];
 #pragma unroll
-  for (int j = 0; j < kVals; ++j) hit[j] = x[j] >= t, n += kLanes == 64 ? (int) __popcll(wave_ballot(hit[j])) : hit[j] ? 1 : 0;
+  for (int j = 0; j < kVals; ++j) {
+    const bool hit = x[j] >= t;
+    n += kLanes == 64 ? (int) __popcll(wave_ballot(hit)) : hit ? 1 : 0;
+    // counted here and now, by an addition that takes the comparison as its carry
+    count[j] = keep_local(count[j] + (hit ? 1 : 0));
+  }
   if (kLanes != 64) n = row_count<kLanes>(n);
+  if (!wave_ballot(n > K)) return;
+  if (wave_ballot(n > 2 * K)) {
+    const bool walk = n > 2 * K;
+    const float counted = as_float((uint32_t) keep_local((int) as_uint(t)));  // or the comparisons' results are kept, in 64 scalar registers
+    float s = unordered(top);
+    for (int r = 1; r < K; ++r) {
+      float below = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < kVals; ++j) count[j] += hit[j] ? 1 : 0;
-  if (wave_ballot(n > K)) {
+      for (int j = 0; j < kVals; ++j) below = fmaxf(below, x[j] < s ? x[j] : -INFINITY);
+      s = unordered(row_max<kLanes>(ordered(below)));
+    }
+    s = fmaxf(s, kLowest);
+    int m = 0;
 #pragma unroll
-    for (int j = 0; j < kVals; ++j) count[j] -= hit[j] ? 1 : 0;
-    if (wave_ballot(n > 2 * K)) {
-      float s = unordered(top);
-      for (int r = 1; r < K; ++r) {
-        float below = -INFINITY;
+    for (int j = 0; j < kVals; ++j) {
+      const bool hit = x[j] >= s;
+      m += kLanes == 64 ? (int) __popcll(wave_ballot(hit)) : hit ? 1 : 0;
+      count[j] -= walk && x[j] >= counted && !hit ? 1 : 0;
+    }
+    if (kLanes != 64) m = row_count<kLanes>(m);
+    if (walk) t = s, n = m;
+  }
+  int left = 0;  // to be chosen of the values equal to t
+  while (wave_ballot(n > K)) {
+    const float gone = n > K ? t : __builtin_nanf("");
+    int equal = 0;
 #pragma unroll
-        for (int j = 0; j < kVals; ++j) below = fmaxf(below, x[j] < s ? x[j] : -INFINITY);
-        s = unordered(row_max<kLanes>(ordered(below)));
+    for (int j = 0; j < kVals; ++j) {
+      const bool hit = x[j] == gone;
+      equal += kLanes == 64 ? (int) __popcll(wave_ballot(hit)) : hit ? 1 : 0;
+      count[j] = keep_local(count[j] - (hit ? 1 : 0));
+    }
+    if (kLanes != 64) equal = row_count<kLanes>(equal);
+    const bool higher = n - equal > K;
+    if (n > K && !higher) left = K - (n - equal);
+    n = higher ? n - equal : 0;
+    if (!wave_ballot(higher)) break;
+    float above = INFINITY;
+#pragma unroll
+    for (int j = 0; j < kVals; ++j) above = fminf(above, x[j] > t ? x[j] : INFINITY);
+    above = unordered(row_min<kLanes>(ordered(above)));
+    if (higher) t = above;
+  }
+  if (kLanes == 64) {
+    // columns rise with the piece, the lane, the value of the piece: over the comparisons' lane masks
+    constexpr int kPiece = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < kVals; i += kPiece) {
+      if (left <= 0) break;
+      unsigned long long equal[kPiece], any = 0;
+#pragma unroll
+      for (int k = 0; k < kPiece; ++k) equal[k] = wave_ballot(x[i + k] == t), any |= equal[k];
+      for (; any && left > 0; any &= any - 1) {
+        const int l = __builtin_ctzll(any);
+#pragma unroll
+        for (int k = 0; k < kPiece; ++k)
+          if (((equal[k] >> l) & 1) && left > 0) {
+            if (lane == 0) atomicAdd(&s_count[column<T, kLanes>(l, i + k)], 1);
+            --left;
+          }
       }
-      s = fmaxf(s, kLowest);
-      const int m = reaching<kLanes, kVals>(x, s);
-      if (n > 2 * K) t = s, n = m;
     }
-    int left = -1;  // of the values equal to t, once fewer than K lie above it
-    while (wave_ballot(n > K && left < 0)) {
-      int greater = 0;
+    return;
+  }
+  for (int at = -1; wave_ballot(left > 0); --left) {
+    const int l = keep_local(lane);  // or every column's index stays in a register of its own
+    int where = 0x7fffffff;
 #pragma unroll
-      for (int j = 0; j < kVals; ++j) greater += kLanes == 64 ? (int) __popcll(wave_ballot(x[j] > t)) : x[j] > t ? 1 : 0;
-      if (kLanes != 64) greater = row_count<kLanes>(greater);
-      const bool higher = n > K && greater >= K;
-      if (n > K && !higher) left = K - greater;
-      if (!wave_ballot(higher)) continue;
-      float above = INFINITY;
-#pragma unroll
-      for (int j = 0; j < kVals; ++j) above = fminf(above, x[j] > t ? x[j] : INFINITY);
-      above = unordered(row_min<kLanes>(ordered(above)));
-      if (higher) t = above, n = greater;
+    for (int j = 0; j < kVals; ++j) {
+      const int c = column<T, kLanes>(l, j);
+      where = min(where, x[j] == t && c > at ? c : 0x7fffffff);
     }
-    if (kLanes == 64 && left > 0) {
-      // columns rise with the piece, the lane, the value of the piece: over the comparisons' lane masks
-      constexpr int kPiece = 16 / sizeof(T);
-#pragma unroll
-      for (int i = 0; i < kVals; i += kPiece) {
-        unsigned long long equal[kPiece], any = 0;
-#pragma unroll
-        for (int k = 0; k < kPiece; ++k) equal[k] = wave_ballot(x[i + k] == t), any |= equal[k];
-        for (; any && left > 0; any &= any - 1) {
-          const int l = __builtin_ctzll(any);
-#pragma unroll
-          for (int k = 0; k < kPiece; ++k)
-            if (((equal[k] >> l) & 1) && left > 0) {
-              if (lane == 0) atomicAdd(&s_count[column<T, kLanes>(l, i + k)], 1);
-              --left;
-            }
-        }
-      }
-      left = 0;
-    }
-    for (int at = -1, more = left; kLanes < 64 && wave_ballot(more > 0); --more) {
-      const int l = keep_local(lane);  // or every column's index stays in a register of its own
-      int where = 0x7fffffff;
-#pragma unroll
-      for (int j = 0; j < kVals; ++j) {
-        const int c = column<T, kLanes>(l, j);
-        where = min(where, x[j] == t && c > at ? c : 0x7fffffff);
-      }
-      at = row_min<kLanes>(where);
-      if (more > 0 && lane == 0) atomicAdd(&s_count[at], 1);
-    }
-    // those above it, above 0 where it is -0; what follows an infinity is a NaN, which nothing reaches
-    if (left >= 0) t = unordered(ordered(t + 0.0f) + 1);
-#pragma unroll
-    for (int j = 0; j < kVals; ++j) count[j] += x[j] >= t ? 1 : 0;
+    at = row_min<kLanes>(where);
+    if (left > 0 && lane == 0) atomicAdd(&s_count[at], 1);
   }
 }
 
