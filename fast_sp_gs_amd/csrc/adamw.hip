@@ -451,15 +451,20 @@ enum Type { kFloat32 = FSGS_DTYPE_F32, kFloat16 = FSGS_DTYPE_F16, kBfloat16 = FS
 size_t type_size(int type) { return type == kFloat32 ? 4 : 2; }
 bool is_type(int type) { return type == kFloat32 || type == kFloat16 || type == kBfloat16; }
 
-// A launch that moves this many bytes goes past the caches: less may still be, or stay, in the 256 MB memory-side cache. us of a step of n
-// elements, three sets of tensors in turn, ordinary and streaming accesses: float32 4M (117 MB) 19.4 and 23.0, 8M 47.2 and 43.6, 16M
-// 91.3 and 84.4, 64M 345 and 324; bfloat16 4M 16.5 and 17.4, 8M (185 MB) 35.3 and 33.4, 64M 267 and 245; 8-bit moments, float32 8M
-// (134 MB) 27.1 and 29.3, 16M 57.1 and 53.1, 64M 198 and 186; read back in bfloat16 16M (101 MB) 17.7 and 20.7, 64M 72.7 and 67.9.
-bool streams(int n, const int64_t* count, size_t bytes_an_element) {
-  constexpr int64_t kStreamBytes = (int64_t) 160 << 20;
+// A launch that moves this many MiB goes past the caches: less may still be, or stay, in the 256 MB memory-side cache. us of a step of n
+// elements, three sets of tensors in turn, ordinary and streaming accesses: float32 4M (117 MB) 18.3 and 21.7, 8M 46.1 and 41.0, 16M
+// 92.1 and 82.2, 64M 351 and 334; bfloat16 4M 15.0 and 16.9, 8M (185 MB) 32.9 and 32.3, 16M 68.7 and 60.7, 64M 270 and 250; 8-bit
+// moments, float32 8M (134 MB) 23.6 and 26.0, 16M 52.3 and 48.6, 64M 193 and 176. One set again and again, with nothing in between, gains by
+// the cache up to 20M elements (16M 65.9 and 79.7), which no training loop does.
+constexpr int kStepMiB = 160;
+// What is read back is mostly writes, which the cache takes in longer: float32 16M (168 MB) 26.1 and 31.4, 28M 45.7 and 50.4, 32M (336 MB)
+// 60.0 and 59.1, 64M 114.7 and 114.0; bfloat16 40M (252 MB) 42.3 and 43.9, 48M 51.2 and 52.6, 64M (403 MB) 73.5 and 68.5. The sum of squares,
+// reads alone, goes by the step's limit.
+constexpr int kReadBackMiB = 320;
+bool streams(int n, const int64_t* count, size_t bytes_an_element, int mib = kStepMiB) {
   int64_t sum = 0;
   for (int q = 0; q < n; ++q) sum += count[q];
-  return sum >= kStreamBytes / (int64_t) bytes_an_element;
+  return sum >= ((int64_t) mib << 20) / (int64_t) bytes_an_element;
 }
 // kernel<type, streaming>
 #define FSGS_BY_TYPE(kernel, dtype, stream)                                                          \
@@ -605,7 +610,7 @@ FSGS_API int fsgs_adamw8_unpack_multi(int n_tensors, int dtype, const int64_t* c
   MomentsTable t{};
   if (const int rc = moments(what, n_tensors, count, state, m, v, type_size(dtype), 4096 / type_size(dtype), t)) return rc;
   if (t.first_block[t.n] == 0) return kOk;
-  auto kernel = FSGS_BY_TYPE(adamw8_unpack_kernel, dtype, streams(n_tensors, count, 2 + 2 * type_size(dtype)));
+  auto kernel = FSGS_BY_TYPE(adamw8_unpack_kernel, dtype, streams(n_tensors, count, 2 + 2 * type_size(dtype), kReadBackMiB));
   hipLaunchKernelGGL(kernel, dim3(t.first_block[t.n]), dim3(256), 0, (hipStream_t) stream, t);
   return check_launch(what);
 }

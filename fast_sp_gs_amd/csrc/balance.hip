@@ -771,8 +771,15 @@ int neighbour_blocks(int64_t N, int64_t M) {
   return (int) std::min(blocks, kNeighbourBlocks / ranges);
 }
 
-// Logits that exceed the 256 MB memory-side cache are read past it.
-bool past_caches(int64_t N, int M, size_t size) { return N >= ((int64_t) 160 << 20) / (int64_t) (M * size); }
+// Logits that exceed the 256 MB memory-side cache are read past it, and their gradients written past it, where a row is made of whole lines of
+// 128 bytes or is long: of lines that two wavefronts share, streaming moves the halves apart. us of forward and backward, ordinary and
+// streaming: float32 320 000 x 512 419 and 367, 1M x 128 341 and 314, 500 000 x 256 360 and 347, 80 000 x 1000 212 and 202, bfloat16 2M x 128
+// 451 and 439; but float32 1M x 100 280 and 320, 600 000 x 200 360 and 376, 500 000 x 300 417 and 444, bfloat16 400 000 x 1000 564 and 576.
+// Rows of 32 values a lane and more are bound by their registers and read either way as fast (100 000 x 2000 173 us both).
+bool past_caches(int64_t N, int M, size_t size) {
+  const int64_t row = (int64_t) (M * size);
+  return N >= ((int64_t) 160 << 20) / row && (row % 128 == 0 || row > 2048);
+}
 
 // kernel<T, lanes, values>(...) for the narrowest rows that hold M columns
 #define FSGS_ROW_KERNELS(T, LAUNCH)                         \
