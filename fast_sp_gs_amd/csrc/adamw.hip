@@ -15,8 +15,9 @@
 //   m  sign, 4 bits of exponent, 3 of fraction: 18 binades
 //   v  5 bits of exponent, 3 of fraction: 34 binades, 17 of the root; a value above 0 is kept above 0, since an element whose
 //      second moment vanished before its first would be divided by eps alone
-// Both are the top of a float32 with a small exponent: decoding shifts the code to that place and scales by a power of two, encoding
-// scales, adds the noise below the last kept bit and shifts, subnormal values of the format included, with no case of its own.
+// Both are the top of a float with a small exponent: decoding shifts the code to its place in a float32 and scales by a power of two; encoding
+// scales a float64, adds the noise below the last kept bit of its upper word and shifts, subnormal values of the format included, with no
+// case of its own.
 // A state is one allocation: codes of m [256 b], codes of v [256 b], exponents (m, v) [b][2] for b blocks. Exponents are those of
 // float32 (biased by 127); 0 is a block of zeros, 255 one that held an infinity or a NaN, all of whose values read as NaN.
 #include <hip/hip_bf16.h>
@@ -123,16 +124,20 @@ __device__ __forceinline__ void store4(T* p, int64_t left, const float in[4]) {
   }
 }
 
+template <typename F>
 struct Step {
-  float b1, b2, c1, c2;  // c = 1 - b
+  F b1, b2, c1, c2;  // c = 1 - b
+};
+// What the norm of the gradients leaves for the step.
+struct Norm {
+  float norm, factor;
+  double exact;  // factor, before it was rounded
 };
 
-// One element; the moments are replaced. The root and the reciprocal are the hardware's, one unit in the last place each. The root's
+// One element, whose moments are the step's already. The root and the reciprocal are the hardware's, one unit in the last place each. The root's
 // instruction takes subnormal numbers for 0, so v counts as 2^-126 at least: the smallest root is 1e-19, a hundred-thousandth of an eps
 // of 1e-15 (scenes' own), and nothing is divided by 0 where eps is. A NaN stays one.
-__device__ __forceinline__ float updated(const Step& s, const Rates& r, float keep, float eps, float p, float g, float& m, float& v) {
-  m = fmaf(s.c1, g, s.b1 * m);
-  v = fmaf(s.c2 * g, g, s.b2 * v);
+__device__ __forceinline__ float updated(const Rates& r, float keep, float eps, float p, float m, float v) {
   const float root = __builtin_amdgcn_sqrtf(v < 0x1p-126f ? 0x1p-126f : v);
   return fmaf(p, keep, -(r.step_size * m * __builtin_amdgcn_rcpf(fmaf(root, r.inv_root_c2, eps))));
 }
@@ -147,25 +152,26 @@ struct Part {
   float* v;
   int64_t count, first;  // first: of the block's elements
   Rates rate;
-  float clip, keep, eps;
+  float keep, eps, factor;
+  double exact_factor;
   bool aligned;  // param and grad, for four elements at once
 
-  __device__ __forceinline__ Part(const AdamwTable& t, const float* factor, const Rates* rates) {
+  __device__ __forceinline__ Part(const AdamwTable& t, const Norm* norm, const Rates* rates) {
     const int q = tensor_of(t.first_block, t.n, blockIdx.x);
     param = (T*) t.param[q], grad = (const T*) t.grad[q], m = t.m[q], v = t.v[q], count = t.count[q];
     first = (int64_t) (blockIdx.x - t.first_block[q]) * 1024;
-    rate = t.rates[q], keep = t.keep[q], eps = t.eps[q], clip = 1.0f;
+    rate = t.rates[q], keep = t.keep[q], eps = t.eps[q], factor = 1.0f, exact_factor = 1.0;
     if (rates) {
       const Rates on_device = rates[q];
       rate = on_device;
     }
-    if (factor) clip = factor[1];
+    if (norm) factor = norm->factor, exact_factor = norm->exact;
     aligned = (((uintptr_t) param | (uintptr_t) grad) & (4 * sizeof(T) - 1)) == 0;
   }
 };
 
 template <typename T, bool kStream, bool kWhole>
-__device__ __forceinline__ void adamw_block(const Part<T>& t, const Step& s) {
+__device__ __forceinline__ void adamw_block(const Part<T>& t, const Step<float>& s) {
   const int64_t e = t.first + threadIdx.x * 4, left = t.count - e;
   if (!kWhole && left <= 0) return;
   float *first = (float*) t.m + e, *second = t.v + e;
@@ -173,16 +179,19 @@ __device__ __forceinline__ void adamw_block(const Part<T>& t, const Step& s) {
   Four<float> m = load4<kWhole, kStream>(first, left), v = load4<kWhole, kStream>(second, left);
   float p[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    p[k] = updated(s, t.rate, t.keep, t.eps, to_float(param.x[k]), t.clip * to_float(grad.x[k]), m.x[k], v.x[k]);
+  for (int k = 0; k < 4; ++k) {
+    const float g = t.factor * to_float(grad.x[k]);
+    m.x[k] = fmaf(s.c1, g, s.b1 * m.x[k]), v.x[k] = fmaf(s.c2 * g, g, s.b2 * v.x[k]);
+    p[k] = updated(t.rate, t.keep, t.eps, to_float(param.x[k]), m.x[k], v.x[k]);
+  }
   store4<kWhole, kStream>(t.param + e, left, p);
   store4<kWhole, kStream>(first, left, m.x), store4<kWhole, kStream>(second, left, v.x);
 }
 
 template <typename T, bool kStream>
-__global__ void __launch_bounds__(256) adamw_kernel(AdamwTable t, Step s, const float* __restrict__ factor,
+__global__ void __launch_bounds__(256) adamw_kernel(AdamwTable t, Step<float> s, const Norm* __restrict__ norm,
                                                     const Rates* __restrict__ rates) {
-  const Part<T> part(t, factor, rates);
+  const Part<T> part(t, norm, rates);
   if (part.aligned && (((uintptr_t) part.m | (uintptr_t) part.v) & 15) == 0 && part.first + 1024 <= part.count)
     adamw_block<T, kStream, true>(part, s);
   else
@@ -210,15 +219,20 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
   return max(max(a, b), max(c, d));
 }
 
+constexpr int kBias = 1023 - 127;  // of a float64's exponent over a float32's
+__device__ __forceinline__ uint32_t upper(double x) { return (uint32_t) (__builtin_bit_cast(uint64_t, x) >> 32); }
+
 // From a code's place in a float32 (exponent 1 is its lowest binade) to that of its block, whose highest one is 2^kBits - 1.
 template <int kBits>  // of exponent
 __device__ __forceinline__ float decoded(uint32_t bits, int exponent) {
   return ldexpf(__builtin_bit_cast(float, bits), exponent + 1 - (1 << kBits));
 }
+// The same the other way round, of a float64, whose upper word has all the bits that count: 3 kept ones and the 16 below them that the noise
+// is added to. What stands below those cannot change the code, so a code is that of the exact value.
 template <int kBits>
-__device__ __forceinline__ uint32_t encoded(float x, int exponent, uint32_t noise16, uint32_t least) {
-  const uint32_t y = __builtin_bit_cast(uint32_t, ldexpf(x, (1 << kBits) - 1 - exponent));
-  return min(max((y + (noise16 << 4)) >> 20, least), (8u << kBits) - 1);
+__device__ __forceinline__ uint32_t encoded(double x, int exponent, uint32_t noise16, uint32_t least) {
+  const uint32_t y = upper(ldexp(x, (1 << kBits) - 1 - kBias - exponent));
+  return min(max((y + (noise16 << 1)) >> 17, least), (8u << kBits) - 1);
 }
 // Element k of the four whose codes are in a word each.
 template <int k>
@@ -239,30 +253,34 @@ __device__ __forceinline__ void decode4(uint32_t codes_m, uint32_t codes_v, int 
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] = __builtin_nanf("");
 }
-// A block's exponent byte from the bits of its largest magnitude (a NaN is larger than any): that of the next binade where the value is
-// above 1.875 of its own. Below the normal numbers the lowest normal exponent stands for all; 254 is the last of finite values.
+// A block's exponent byte from the upper word of its largest magnitude (a NaN is larger than any; the last bit stands for all bits
+// of the lower word): that of the next binade where the value is above 1.875 of its own. What float32 cannot hold is an infinity or 0. Below the
+// normal numbers the lowest normal exponent stands for all; 254 is the last of finite values.
 __device__ __forceinline__ int block_exponent(uint32_t top) {
-  if (top >= 0x7f800000u) return 255;
-  return top ? min(max((int) ((top + 0xfffffu) >> 23), 1), 254) : 0;
+  if (top >= (uint32_t) (kBias + 255) << 20) return 255;
+  if (top < (uint32_t) (kBias + 1 - 23) << 20) return 0;
+  return min(max((int) ((top + 0x1ffffu) >> 20) - kBias, 1), 254);
+}
+__device__ __forceinline__ uint32_t magnitude(double x) {
+  return (upper(x) & 0x7fffffffu) | min((uint32_t) __builtin_bit_cast(uint64_t, x), 1u);
 }
 
-// Codes of four elements of a block, and the block's exponents; the noise of m in the low half of a word, of v in the high one.
-__device__ __forceinline__ void encode4(const float m[4], const float v[4], const uint32_t noise[4], uint32_t& codes_m,
+// Codes of four elements of a block, and the block's exponents; the noise of m in the low half of a word, of v in the high one. The moments come
+// in 64 bits: rounded to 32 before, one value in a million falls on the other side of a border, and equal inputs give other codes than the
+// definition does. Ten more operations an element, at the rate of 32-bit ones: 64M elements in float32 179 us against 174, in bfloat16 152
+// against 143.
+__device__ __forceinline__ void encode4(const double m[4], const double v[4], const uint32_t noise[4], uint32_t& codes_m,
                                         uint32_t& codes_v, int& exponent_m, int& exponent_v) {
   uint32_t top_m = 0, top_v = 0;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    top_m = max(top_m, __builtin_bit_cast(uint32_t, m[k]) & 0x7fffffffu);
-    top_v = max(top_v, __builtin_bit_cast(uint32_t, v[k]) & 0x7fffffffu);
-  }
+  for (int k = 0; k < 4; ++k) top_m = max(top_m, magnitude(m[k])), top_v = max(top_v, magnitude(v[k]));
   exponent_m = block_exponent(wave_max(top_m)), exponent_v = block_exponent(wave_max(top_v));
   codes_m = codes_v = 0;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const uint32_t bits_m = __builtin_bit_cast(uint32_t, m[k]), bits_v = __builtin_bit_cast(uint32_t, v[k]);
-    const uint32_t a = encoded<4>(fabsf(m[k]), exponent_m, noise[k] & 0xffffu, 0);
-    const uint32_t b = encoded<5>(v[k], exponent_v, noise[k] >> 16, min(bits_v, 1u));
-    codes_m |= (a | ((bits_m >> 24) & 128u)) << (8 * k);
+    const uint32_t a = encoded<4>(fabs(m[k]), exponent_m, noise[k] & 0xffffu, 0);
+    const uint32_t b = encoded<5>(v[k], exponent_v, noise[k] >> 16, (float) v[k] > 0.0f ? 1 : 0);
+    codes_m |= (a | ((upper(m[k]) >> 24) & 128u)) << (8 * k);
     codes_v |= b << (8 * k);
   }
 }
@@ -278,20 +296,23 @@ __host__ __device__ __forceinline__ StateView view_state(void* state, int64_t co
 
 // A wavefront steps a block: a lane has four elements of it.
 template <typename T, bool kStream, bool kWhole>
-__device__ __forceinline__ void adamw8_block(const Part<T>& t, const Step& s, int64_t block) {
+__device__ __forceinline__ void adamw8_block(const Part<T>& t, const Step<double>& s, int64_t block) {
   const int lane = threadIdx.x & 63;
   const int64_t e = block * kBlock + lane * 4, left = t.count - e;
   const StateView state = view_state(t.m, t.count);
   const Four<T> param = load4<kWhole, kStream>(t.param + e, left), grad = load4<kWhole, kStream>(t.grad + e, left);
   uint32_t codes_m = get<kStream, uint32_t>(state.m + e), codes_v = get<kStream, uint32_t>(state.v + e);
   const int exponents = __builtin_amdgcn_readfirstlane(*(const uint16_t*) (state.exponents + 2 * block));
-  float m[4], v[4], p[4];
+  float old_m[4], old_v[4], p[4];
+  double m[4], v[4];
   uint32_t noise[4];
-  decode4(codes_m, codes_v, exponents & 255, exponents >> 8, m, v);
+  decode4(codes_m, codes_v, exponents & 255, exponents >> 8, old_m, old_v);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    p[k] = updated(s, t.rate, t.keep, t.eps, to_float(param.x[k]), t.clip * to_float(grad.x[k]), m[k], v[k]);
-    if (!kWhole && k >= left) m[k] = v[k] = 0.0f;
+    const double g = t.exact_factor * (double) to_float(grad.x[k]);
+    m[k] = fma(s.c1, g, s.b1 * (double) old_m[k]), v[k] = fma(s.c2 * g, g, s.b2 * (double) old_v[k]);
+    p[k] = updated(t.rate, t.keep, t.eps, to_float(param.x[k]), (float) m[k], (float) v[k]);
+    if (!kWhole && k >= left) m[k] = v[k] = 0.0;
     noise[k] = mixed((uint32_t) (e + k) * kStride + t.rate.key);
   }
   int exponent_m, exponent_v;
@@ -302,9 +323,9 @@ __device__ __forceinline__ void adamw8_block(const Part<T>& t, const Step& s, in
 }
 
 template <typename T, bool kStream>
-__global__ void __launch_bounds__(256) adamw8_kernel(AdamwTable t, Step s, const float* __restrict__ factor,
+__global__ void __launch_bounds__(256) adamw8_kernel(AdamwTable t, Step<double> s, const Norm* __restrict__ norm,
                                                      const Rates* __restrict__ rates) {
-  const Part<T> part(t, factor, rates);
+  const Part<T> part(t, norm, rates);
   const int64_t block = part.first / kBlock + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (block * kBlock >= part.count) return;  // the whole wavefront
   if (part.aligned && (block + 1) * kBlock <= part.count) adamw8_block<T, kStream, true>(part, s, block);
@@ -360,9 +381,10 @@ __global__ void __launch_bounds__(256) adamw8_pack_kernel(MomentsTable t) {
   const StateView state = view_state(t.state[q], t.count[q]);
   const Four<float> m = load4<false, false>((const float*) t.m[q] + e, left), v = load4<false, false>((const float*) t.v[q] + e, left);
   const uint32_t noise[4] = {0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
+  const double exact_m[4] = {m.x[0], m.x[1], m.x[2], m.x[3]}, exact_v[4] = {v.x[0], v.x[1], v.x[2], v.x[3]};
   uint32_t codes_m, codes_v;
   int exponent_m, exponent_v;
-  encode4(m.x, v.x, noise, codes_m, codes_v, exponent_m, exponent_v);
+  encode4(exact_m, exact_v, noise, codes_m, codes_v, exponent_m, exponent_v);
   *(uint32_t*) (state.m + e) = codes_m, *(uint32_t*) (state.v + e) = codes_v;
   if (lane == 0) *(uint16_t*) (state.exponents + 2 * block) = (uint16_t) (exponent_m | exponent_v << 8);
 }
@@ -384,49 +406,47 @@ __device__ __forceinline__ double block_sum(double x, double* s_wave) {
   return ((s_wave[0] + s_wave[1]) + s_wave[2]) + s_wave[3];
 }
 
-// Sums of squares: a lane's 32 elements of a chunk in float32 (four sums of eight), everything above in float64.
+// Sums of squares, in float64 from the first element on: its multiply-adds go at the rate of float32's, and the pass waits for memory.
 template <typename T, bool kStream>
 __global__ void __launch_bounds__(256) square_sums_kernel(NormTable t, double* __restrict__ sums) {
   __shared__ double s_wave[4];
-  double total = 0.0;
+  double sum[4] = {0.0, 0.0, 0.0, 0.0};
+  const auto add = [&](const Four<T>& g) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const double x = (double) to_float(g.x[k]);
+      sum[k] = fma(x, x, sum[k]);
+    }
+  };
   for (unsigned chunk = blockIdx.x; chunk < t.first_chunk[t.n]; chunk += gridDim.x) {
     const int q = tensor_of(t.first_chunk, t.n, chunk);
     const int64_t at = (int64_t) (chunk - t.first_chunk[q]) * kNormChunk + threadIdx.x * 4, count = t.count[q];
     const T* grad = (const T*) t.grad[q];
     const bool aligned = ((uintptr_t) grad & (4 * sizeof(T) - 1)) == 0;
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (aligned && (int64_t) (chunk - t.first_chunk[q] + 1) * kNormChunk <= count) {
       Four<T> g[kNormChunk / 1024];
 #pragma unroll
       for (int j = 0; j < kNormChunk / 1024; ++j) g[j] = load4<true, kStream>(grad + at + j * 1024, 4);
 #pragma unroll
-      for (int j = 0; j < kNormChunk / 1024; ++j)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) sum[k] = fmaf(to_float(g[j].x[k]), to_float(g[j].x[k]), sum[k]);
+      for (int j = 0; j < kNormChunk / 1024; ++j) add(g[j]);
     } else {
-      for (int64_t e = at; e < count && e < at + kNormChunk; e += 1024) {
-        const Four<T> g = load4<false, kStream>(grad + e, count - e);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) sum[k] = fmaf(to_float(g.x[k]), to_float(g.x[k]), sum[k]);
-      }
+      for (int64_t e = at; e < count && e < at + kNormChunk; e += 1024) add(load4<false, kStream>(grad + e, count - e));
     }
-    total += ((double) sum[0] + sum[1]) + ((double) sum[2] + sum[3]);
   }
-  total = block_sum(total, s_wave);
+  const double total = block_sum((sum[0] + sum[1]) + (sum[2] + sum[3]), s_wave);
   if (threadIdx.x == 0) sums[blockIdx.x] = total;
 }
 
-__global__ void __launch_bounds__(256) norm_factor_kernel(int n, const double* __restrict__ sums, double max_norm,
-                                                          float* __restrict__ out) {
+__global__ void __launch_bounds__(256) norm_factor_kernel(int n, const double* __restrict__ sums, double max_norm, Norm* __restrict__ out) {
   __shared__ double s_wave[4];
   double total = 0.0;
   for (int k = threadIdx.x; k < n; k += 256) total += sums[k];
   total = block_sum(total, s_wave);
   if (threadIdx.x != 0) return;
-  const float norm = (float) sqrt(total);
-  const float factor = (float) max_norm / (norm + 1e-6f);
+  const double norm = sqrt(total), factor = max_norm / (norm + 1e-6);
   // a NaN passes, as a comparison with it would not let it
-  out[0] = norm, out[1] = factor > 1.0f ? 1.0f : factor;
+  const double exact = factor > 1.0 ? 1.0 : factor;
+  *out = Norm{(float) norm, (float) exact, exact};
 }
 
 // ---- step counts on the device ------------------------------------------------------------------------------------------------
@@ -516,9 +536,11 @@ FSGS_API int fsgs_grad_square_sums(int n_tensors, int dtype, const int64_t* coun
   return check_launch(what);
 }
 
+FSGS_API size_t fsgs_grad_norm_bytes(void) { return sizeof(Norm); }
 FSGS_API int fsgs_grad_norm_factor(int n_sums, const double* sums, double max_norm, float* norm_and_factor, void* stream) {
   FSGS_REQUIRE(n_sums >= 0 && (n_sums == 0 || sums) && norm_and_factor, "grad_norm: null pointer");
-  hipLaunchKernelGGL(norm_factor_kernel, dim3(1), dim3(256), 0, (hipStream_t) stream, n_sums, sums, max_norm, norm_and_factor);
+  FSGS_REQUIRE((uintptr_t) norm_and_factor % 8 == 0, "grad_norm: misaligned address");
+  hipLaunchKernelGGL(norm_factor_kernel, dim3(1), dim3(256), 0, (hipStream_t) stream, n_sums, sums, max_norm, (Norm*) norm_and_factor);
   return check_launch("grad_norm");
 }
 
@@ -566,10 +588,17 @@ int adamw_update(const char* what, int bits, int n, int dtype, const int64_t* co
     t.rates[q].inv_root_c2 = inv_root_c2;
     t.rates[q].key         = noise_key((uint32_t) (int64_t) known, seed);
   }
-  const Step s{(float) b1, (float) b2, (float) (1.0 - b1), (float) (1.0 - b2)};
+  FSGS_REQUIRE((uintptr_t) factor % 8 == 0, "%s: misaligned address", what);
+  const Norm* norm = (const Norm*) factor;
   const bool past = streams(n, count, 3 * type_size(dtype) + (bits == 8 ? 4 : 16));
-  auto kernel = bits == 8 ? FSGS_BY_TYPE(adamw8_kernel, dtype, past) : FSGS_BY_TYPE(adamw_kernel, dtype, past);
-  hipLaunchKernelGGL(kernel, dim3(t.first_block[n]), dim3(256), 0, (hipStream_t) stream, t, s, factor, (const Rates*) rates);
+  const dim3 grid(t.first_block[n]);
+  if (bits == 8) {
+    const Step<double> s{b1, b2, 1.0 - b1, 1.0 - b2};
+    hipLaunchKernelGGL(FSGS_BY_TYPE(adamw8_kernel, dtype, past), grid, dim3(256), 0, (hipStream_t) stream, t, s, norm, (const Rates*) rates);
+  } else {
+    const Step<float> s{(float) b1, (float) b2, (float) (1.0 - b1), (float) (1.0 - b2)};
+    hipLaunchKernelGGL(FSGS_BY_TYPE(adamw_kernel, dtype, past), grid, dim3(256), 0, (hipStream_t) stream, t, s, norm, (const Rates*) rates);
+  }
   return check_launch(what);
 }
 

@@ -110,7 +110,8 @@ struct Call {
     refuse_twice(w, "parameter", params), refuse_twice(w, "step count", steps);
     if (has(norm)) {
       require(what, "norm", *norm, at::kFloat), require_device(w, "norm", *norm, device);
-      if (norm->numel() != 2) fail(w + ": norm must be what grad_norm returned");
+      const int64_t room = (int64_t) norm->storage().nbytes() - norm->storage_offset() * 4;
+      if (norm->numel() != 2 || room < (int64_t) fsgs_grad_norm_bytes() || (uintptr_t) norm->data_ptr() % 8) fail(w + ": norm must be what grad_norm returned");
     }
     for (size_t k = 0; k < n; ++k)
       grads.push_back(alike(given[k], params[k]) ? given[k] : at::empty_like(params[k]).copy_(given[k]));
@@ -168,7 +169,8 @@ Tensor grad_norm(const std::vector<Tensor>& grads, double max_norm) {
   const c10::DeviceGuard guard(device);
   const Launches launches(what, "grad", dense);
   const int each = std::max(64, fsgs_grad_square_sums_max() / (int) launches.list.size());
-  const Tensor sums = empty({each * (int64_t) launches.list.size()}, dense[0], at::kDouble), out = empty({2}, dense[0]);
+  const Tensor sums = empty({each * (int64_t) launches.list.size()}, dense[0], at::kDouble);
+  const Tensor out = part_of(empty({(int64_t) fsgs_grad_norm_bytes()}, dense[0], at::kByte), 0, {2}, {1}, at::kFloat);
   void* stream = stream_of(dense[0]);
   double* at = data<double>(sums);
   for (const auto& [code, which] : launches.list) {

@@ -990,7 +990,7 @@ int fsgs_adam_masked_update_multi(int n_tensors, int64_t N, const int64_t* M, co
 /* p = p (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps) after m = b1 m + (1 - b1) c g, v = b2 v + (1 - b2) (c g)^2,
  * for up to fsgs_adamw_max_tensors() tensors of count[q] elements in one launch. Host arrays with one entry per tensor: count, step (t, the
  * one that is being taken), lr, eps, decay and the addresses. dtype (FSGS_DTYPE_F32, _F16, _BF16) is that of param and grad; m and v are
- * float32. norm_and_factor (device, optional): what fsgs_grad_norm_factor wrote, c = norm_and_factor[1]; 1 without it.
+ * float32. norm_and_factor (device, optional): what fsgs_grad_norm_factor wrote; c is 1 without it.
  * rates (device, optional): what fsgs_adamw_rates wrote for the same tensors; step may be NULL then. Addresses need the alignment of
  * their element type; those of four elements are moved in one access. A launch takes fewer than 2^34 elements. */
 int fsgs_adamw_max_tensors(void);
@@ -998,8 +998,8 @@ int fsgs_adamw_update_multi(int n_tensors, int dtype, const int64_t* count, cons
     double b2, const double* eps, const double* decay, const void* rates, const float* norm_and_factor, void* const* param,
     const void* const* grad, float* const* m, float* const* v, void* stream);
 /* The same with both moments in 8 bits: state[q] has fsgs_adamw8_state_bytes(count[q]) bytes, 16-byte aligned, all zero before the first
- * step. Blocks of 256 elements under one exponent per moment, the codes rounded by a hash of (element, step, seed) so that they are
- * right on average; an infinity or a NaN among a block's moments makes all of the block's NaN. */
+ * step. Blocks of 256 elements under one exponent per moment; the moments are formed in float64, and their codes rounded by a hash of
+ * (element, step, seed) so that they are right on average; an infinity or a NaN among a block's moments makes all of the block's NaN. */
 size_t fsgs_adamw8_state_bytes(int64_t count);
 int fsgs_adamw8_update_multi(int n_tensors, int dtype, const int64_t* count, const double* step, const double* lr, double b1,
     double b2, const double* eps, const double* decay, uint32_t seed, const void* rates, const float* norm_and_factor,
@@ -1016,7 +1016,9 @@ int fsgs_adamw_rates(int n_tensors, float* const* step, const double* lr, double
     void* stream);
 /* The norm of all gradients together: fsgs_grad_square_sums writes n_sums (at most fsgs_grad_square_sums_max()) sums of the squares of
  * up to fsgs_adamw_max_tensors() tensors, fsgs_grad_norm_factor turns the sums of all its calls, one behind the other, into
- * norm_and_factor[2] = {norm, min(1, max_norm / (norm + 1e-6))}. */
+ * norm_and_factor (fsgs_grad_norm_bytes() bytes, 8-byte aligned): the floats {norm, min(1, max_norm / (norm + 1e-6))}, then the latter as a
+ * double, which the 8-bit step takes. */
+size_t fsgs_grad_norm_bytes(void);
 int fsgs_grad_square_sums_max(void);
 int fsgs_grad_square_sums(int n_tensors, int dtype, const int64_t* count, const void* const* grad, int n_sums, double* sums,
     void* stream);

@@ -518,3 +518,26 @@ def test_more_elements_than_a_launch_takes_are_refused(device):
     with pytest.raises(RuntimeError, match='elements'):
         adamw8_step([p], [p], [state], [step])
     assert float(step) == 0.0
+
+
+@pytest.mark.parametrize('clip', [False, True])
+def test_codes_are_those_of_the_exact_moments(device, clip):
+    """Values that lie within a float32's rounding of a border fall on the side that the definition puts them on: not one of a million
+    codes differs (in float64 both sides are off by parts in 10^16, a border is that near for none of them)."""
+    from fast_sp_gs_amd.adamw import adamw8_pack, adamw8_step
+    n = 1 << 18
+    params, grads, ms, vs, steps = _problem(device, [n, n], torch.float32, 31)
+    states = adamw8_pack(ms, vs)
+    old = [R.unpack(npy(s), n) for s in states]
+    total = np.sqrt(sum((_flat(g) ** 2).sum() for g in grads))
+    factor = min(1.0, 0.3 * total / (total + 1e-6)) if clip else 1.0
+    adamw8_step(params, grads, states, steps, max_norm=0.3 * total if clip else None, seed=8)
+    for k in range(2):
+        t = int(steps[k])
+        _, m, v, _ = R.step64(0.0, _flat(grads[k]), *old[k], t, 1e-3, factor=factor)
+        got_m, got_v = R.unpack(npy(states[k]), n)
+        u_m, u_v = R.noise(n, t, 8)
+        kept_m, _ = R.rounded(abs(m), u_m, 4)
+        kept_v, spacing = R.rounded(v, u_v, 5)
+        assert np.array_equal(got_m, np.sign(m) * kept_m)
+        assert np.array_equal(got_v, np.where((kept_v == 0) & (v > 0), spacing, kept_v))
