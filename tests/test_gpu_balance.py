@@ -95,6 +95,19 @@ def test_loss_counts_and_gradient(device, N, M, dtype):
         _check(x.to(device), K, None if rows is None else rows.to(device), r, dtype, (0.7, up))
 
 
+@pytest.mark.parametrize('N,M,dtype', [(1000, 4500, torch.float32), (900, 8192, torch.bfloat16), (7, 8193, torch.float32), (5, 16384, torch.float16),
+                                       (4, 16385, torch.float32), (3, 20001, torch.bfloat16)])
+def test_rows_that_take_a_block(device, N, M, dtype):
+    """More superpoints than a wavefront's lanes hold, blocks with a second row, with ties and with points left out."""
+    g = torch.Generator().manual_seed(M)
+    x = (torch.randn(N, M, generator=g) * 2).round(decimals=1).to(dtype)
+    rows = torch.rand(N, generator=g) < 0.8
+    rows[0] = True
+    for K in (1, 5):
+        r = _reference(x.double().numpy(), K, npy(rows))
+        _check(x.to(device), K, rows.to(device), r, dtype, (0.7, torch.randn(M, generator=g).to(device)))
+
+
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize('M', [7, 16, 64, 100, 512, 1030, 4097])
 def test_ties_go_to_the_lowest_index(device, M, dtype):
