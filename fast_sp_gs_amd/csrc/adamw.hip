@@ -143,6 +143,9 @@ __device__ __forceinline__ float updated(const Rates& r, float keep, float eps, 
 }
 
 // ---- 32-bit moments -------------------------------------------------------------------------------------------------------------
+// A block steps 1024 elements of one tensor, found by a binary search in the table that the launch carries: one launch whatever the tensors'
+// number and sizes, no job list in memory. 28 bytes an element in float32 (22 in 16 bits) for some fifteen operations: memory. 174M elements
+// of six tensors 805 - 821 us (6.0 TB/s), 8M in bfloat16 29 us, 0.5M in 25 tensors 5.1 us, which is the launch and two dependent loads.
 // What a block needs of its tensor, in scalar registers.
 template <typename T>
 struct Part {
@@ -199,6 +202,9 @@ __global__ void __launch_bounds__(256) adamw_kernel(AdamwTable t, Step<float> s,
 }
 
 // ---- 8-bit moments ----------------------------------------------------------------------------------------------------------------
+// 16 bytes an element in float32 (10 in 16 bits), the exponents 4 in 256: memory in float32, 171M elements 432 - 447 us (6.1 - 6.3 TB/s). In 16 bits
+// decoding, the step, the hash and encoding take longer than the accesses: 8M in bfloat16 24 us (3.3 TB/s), 21 with ten operations an element
+// less. Two blocks for each wavefront were slower.
 __host__ __device__ __forceinline__ uint32_t mixed(uint32_t x) {
   x = (x ^ (x >> 16)) * 0xBB67AE85u;
   x = (x ^ (x >> 15)) * 0x3C6EF373u;
@@ -341,7 +347,7 @@ struct MomentsTable {
   int n;
 };
 
-// The values that 8-bit moments stand for; a lane writes 16 bytes of each.
+// The values that 8-bit moments stand for; a lane writes 16 bytes of each. 171M elements in bfloat16 162 us (6.3 TB/s), 8M 10.5 us.
 template <typename T, bool kStream>
 __global__ void __launch_bounds__(256) adamw8_unpack_kernel(MomentsTable t) {
   constexpr int kWords = 4 / sizeof(T);  // of four codes
@@ -406,7 +412,8 @@ __device__ __forceinline__ double block_sum(double x, double* s_wave) {
   return ((s_wave[0] + s_wave[1]) + s_wave[2]) + s_wave[3];
 }
 
-// Sums of squares, in float64 from the first element on: its multiply-adds go at the rate of float32's, and the pass waits for memory.
+// Sums of squares, in float64 from the first element on: its multiply-adds go at the rate of float32's, and the pass waits for memory. A
+// chunk's eight loads are on their way together. 174M float32 104 us (6.7 TB/s), 8M bfloat16 9 us.
 template <typename T, bool kStream>
 __global__ void __launch_bounds__(256) square_sums_kernel(NormTable t, double* __restrict__ sums) {
   __shared__ double s_wave[4];
