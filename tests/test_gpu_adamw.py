@@ -541,3 +541,33 @@ def test_codes_are_those_of_the_exact_moments(device, clip):
         kept_v, spacing = R.rounded(v, u_v, 5)
         assert np.array_equal(got_m, np.sign(m) * kept_m)
         assert np.array_equal(got_v, np.where((kept_v == 0) & (v > 0), spacing, kept_v))
+
+
+def test_a_moment_that_equals_its_gradient_stays(device):
+    """Codes' own values as gradients, with every noise there is (0 among them): m and v are on their codes' borders and keep them."""
+    from fast_sp_gs_amd.adamw import adamw8_pack, adamw8_step
+    n = 1 << 20
+    values = torch.tensor([1.0, 1.125, 0.625, 0.01171875], device=device).repeat(n // 4)
+    p, step = torch.zeros(n, device=device), torch.tensor(3.0)
+    m, = adamw8_pack([values], [torch.ones_like(values)])
+    before = m.clone()
+    adamw8_step([p], [values.clone()], [m], [step], lr=0.0, betas=(0.9, 0.0))
+    assert torch.equal(m[:n], before[:n])
+    ones = torch.tensor([1.0, 0.5, 2.0, 0.25], device=device).repeat(n // 4)
+    state, = adamw8_pack([ones], [ones * ones])
+    before = state.clone()
+    for seed in range(4):
+        adamw8_step([p], [ones], [state], [step], lr=0.0, seed=seed)
+        assert torch.equal(state, before)
+
+
+def test_moments_on_a_border_by_decimal_betas(device):
+    """0.9 * 9 / 8 + 0.1 * 8 is 14.5 / 8: with a noise of a half it reaches 15 / 8, though 1 - 0.9 in binary falls short of 0.1 by 2e-17."""
+    from fast_sp_gs_amd.adamw import adamw8_pack, adamw8_step
+    n = 1 << 20
+    p, m = torch.zeros(n, device=device), torch.full((n,), 9 / 8, device=device)
+    state, = adamw8_pack([m], [torch.ones(n, device=device)])
+    adamw8_step([p], [torch.full((n,), 8.0, device=device)], [state], [torch.tensor(5.0)], lr=0.0, seed=2)
+    u, _ = R.noise(n, 6, 2)
+    assert (u == 0.5).any()
+    assert np.array_equal(R.unpack(npy(state), n)[0], np.where(u >= 0.5, 15 / 8, 14 / 8))
