@@ -272,10 +272,11 @@ __device__ __forceinline__ void choose(const float x[kVals], int lane_top, int t
 }
 
 // exp(x - shift) of the row's values. The shift's product with log2 e is rounded once for the whole row, a factor that the row's sum has too:
-// one multiply-add a value. Where the product could overflow the difference is taken first.
+// one multiply-add a value. That factor is 2 to half an ulp of the product: within 2^(1/16) up to a shift of 2^20, beyond float32 from 2^32 on
+// (2^440 in a row of -1e10). From 2^20 on the difference is taken first.
 template <int kVals>
 __device__ __forceinline__ void exponentials(float x[kVals], float shift) {
-  const bool far = fabsf(shift) > 1e38f;
+  const bool far = fabsf(shift) >= 0x1p20f;
   if (wave_ballot(far)) {
 #pragma unroll
     for (int j = 0; j < kVals; ++j) x[j] = far ? x[j] - shift : x[j];

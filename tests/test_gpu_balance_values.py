@@ -1,0 +1,37 @@
+"""Balance losses of logits far from 0 and of zeros of both signs, in every width of row, against their definition in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_balance import _check, _reference
+
+pytestmark = pytest.mark.gpu
+
+# every number of lanes and of values a lane, whole rows and rows that end inside them
+WIDTHS = [7, 16, 31, 64, 100, 128, 200, 256, 500, 512, 1000, 1500, 2048, 2500, 4096, 4097]
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('M', WIDTHS)
+def test_logits_of_any_magnitude(device, M, dtype):
+    """Rows about a large value of either sign: all equal, one ahead of the others, some steps of the type apart; and as a mask, over a part
+    of a row or the whole of it. Tolerances are those of ordinary rows: differences from the row's largest logit are what counts."""
+    g = torch.Generator().manual_seed(M)
+    x = []
+    for size in (1e5, 1e6, 1.1e6, 1e8, 3e9, 1e10, 1e20, 1e30, 9e37, 1.1e38, 3e38):
+        for v in (size, -size):
+            at = torch.tensor(v).to(dtype).float()
+            equal = at.expand(M).clone()
+            ahead = equal * (0.9375 if v > 0 else 1.0625)
+            ahead[M // 3] = at
+            apart = at * (1 + torch.randint(-3, 4, (M,), generator=g) * float(torch.finfo(dtype).eps))
+            masked = torch.randn(M, generator=g)
+            masked[torch.rand(M, generator=g) < 0.5] = -abs(at)
+            x += [equal, ahead, apart, masked]
+    x = torch.stack(x).to(dtype)
+    assert torch.isfinite(x).all()
+    N = len(x)
+    rows = torch.rand(N, generator=g) < 0.8
+    for K, on in ((1, None), (3, rows)):
+        r = _reference(x.double().numpy(), K, np.ones(N, bool) if on is None else on.numpy())
+        _check(x.to(device), K, None if on is None else on.to(device), r, dtype, (0.7, torch.randn(M, generator=g).to(device)))
