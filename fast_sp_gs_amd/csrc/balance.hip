@@ -321,7 +321,9 @@ __global__ void __launch_bounds__(row_threads(kVals), row_waves(kVals)) balance_
     float lane_top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < kVals; ++j) lane_top = fmaxf(lane_top, x[j]);
-    const int lane_top_ordered = ordered(lane_top), top_ordered = row_max<kLanes>(lane_top_ordered);
+    // -0 becomes +0, to which it compares equal: as integers they would be two values, and the K-th of the lanes' largest, which sets the first
+    // threshold, could lie above the K-th value of the row
+    const int lane_top_ordered = ordered(lane_top + 0.0f), top_ordered = row_max<kLanes>(lane_top_ordered);
     choose<T, kLanes, kVals>(x, lane_top_ordered, top_ordered, K, lane, count, s_count);
     // a row without a number (top is -inf): the sum is 0, or NaN where one of its values is, which counts
     const float top = unordered(top_ordered), shift = top == -INFINITY ? 0.0f : top;

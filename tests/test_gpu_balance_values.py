@@ -35,3 +35,18 @@ def test_logits_of_any_magnitude(device, M, dtype):
     for K, on in ((1, None), (3, rows)):
         r = _reference(x.double().numpy(), K, np.ones(N, bool) if on is None else on.numpy())
         _check(x.to(device), K, None if on is None else on.to(device), r, dtype, (0.7, torch.randn(M, generator=g).to(device)))
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('M', WIDTHS)
+def test_zeros_of_both_signs_are_equal(device, M, dtype):
+    """Negative logits, many of them multiplied by 0: -0 and +0 tie, the lowest index first, whichever sign the lanes' largest have."""
+    g = torch.Generator().manual_seed(M + 1)
+    N = 48
+    x = -torch.rand(N, M, generator=g) - 0.01
+    kept = torch.rand(N, M, generator=g) < torch.linspace(0, 1, N)[:, None]
+    zero = torch.where(torch.rand(N, M, generator=g) < torch.tensor([0.0, 0.02, 0.5, 1.0]).repeat(N // 4)[:, None], 0.0, -0.0)
+    x = torch.where(kept, x, zero).to(dtype)
+    for K in (1, 2, 3, 4, 5, 7):
+        r = _reference(x.double().numpy(), K, np.ones(N, bool))
+        _check(x.to(device), K, None, r, dtype)
