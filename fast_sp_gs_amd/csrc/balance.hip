@@ -402,6 +402,11 @@ __global__ void __launch_bounds__(256) balance_rows_backward_kernel(int64_t N, i
     const int c = column<T, kLanes>(lane, j);
     slope[j] = c < M ? of_counts * (float) counts[c] + (g_importance ? g_importance[c] / rows : 0.0f) : 0.0f;
   }
+  // weights of 0 do not make 0 of slopes that are no numbers
+  bool finite = true;
+#pragma unroll
+  for (int j = 0; j < kVals; ++j) finite = finite && fabsf(slope[j]) < INFINITY;
+  const bool any_odd = wave_ballot(!finite) != 0;
   const int64_t step = (int64_t) gridDim.x * 4 * kRows;
   int64_t base = ((int64_t) blockIdx.x * 4 + wave) * kRows;
 
@@ -418,13 +423,18 @@ __global__ void __launch_bounds__(256) balance_rows_backward_kernel(int64_t N, i
     for (int j = 0; j < kVals; ++j) x[j] *= stat.y, mean = fmaf(x[j], slope[j], mean);
     mean = row_sum<kLanes>(mean);
     if (at >= N) return;
+#pragma unroll
+    for (int j = 0; j < kVals; ++j) x[j] *= slope[j] - mean;
+    if (any_odd)
+#pragma unroll
+      for (int j = 0; j < kVals; ++j) x[j] = on ? x[j] : 0.0f;
     T* out = grad + at * M;
 #pragma unroll
     for (int j = 0; j < kVals; j += kPiece) {
       const int c = column<T, kLanes>(lane, j);
       Pack<T, kPiece> q;
 #pragma unroll
-      for (int k = 0; k < kPiece; ++k) from_float(x[j + k] * (slope[j + k] - mean), q.x[k]);
+      for (int k = 0; k < kPiece; ++k) from_float(x[j + k], q.x[k]);
       if (kAccess == kStream) {
         typedef uint32_t Raw __attribute__((ext_vector_type(4)));
         if (c < M) __builtin_nontemporal_store(__builtin_bit_cast(Raw, q), (Raw*) (out + c));

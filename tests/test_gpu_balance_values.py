@@ -50,3 +50,24 @@ def test_zeros_of_both_signs_are_equal(device, M, dtype):
     for K in (1, 2, 3, 4, 5, 7):
         r = _reference(x.double().numpy(), K, np.ones(N, bool))
         _check(x.to(device), K, None, r, dtype)
+
+
+@pytest.mark.parametrize('M', WIDTHS)
+def test_rows_that_do_not_count_have_no_gradient(device, M):
+    """Whatever comes from above: a NaN or an infinity in the importance's gradient reaches the rows that count and no other."""
+    from fast_sp_gs_amd.balance import balance_loss
+    g = torch.Generator().manual_seed(M + 2)
+    N = 40
+    x = torch.randn(N, M, generator=g).to(device)
+    x[5] = float('-inf')
+    rows = torch.rand(N, generator=g) < 0.6
+    rows[:6] = True
+    on = rows.clone()
+    on[5] = False
+    x.requires_grad_(True)
+    for bad in (float('nan'), float('inf')):
+        up = torch.zeros(M, device=device)
+        up[M // 2] = bad
+        grad, = torch.autograd.grad(balance_loss(x, 2, rows.to(device))[2], x, up)
+        assert not bool(grad[(~on).to(device)].any())
+        assert not bool(torch.isfinite(grad[on.to(device)]).any())
