@@ -9,7 +9,7 @@ tests can compare its gradients with other formulations.
 
 With neighbour logits `sp_W` [N, M] (LBS_method 'W', network.py:514-515) the association of points to control points is learned too, held
 apart by `balance` times the balance loss of the logits; `weight_decay`, `state_bits` and `max_norm` have the network, the control points
-and the logits stepped by `AdamW` instead of plain Adam.
+and the logits stepped by `AdamW` instead of plain Adam; the network's weights alone decay.
 
 The network runs on the bf16 copies of its weights that it made when it was first called, since the network's plain optimiser
 leaves the parameters' version counters alone, as torch's fused Adam does: a training loop calls `step.net.pack()` after
@@ -56,8 +56,9 @@ class DynamicStep:
         if sp_W is None and not weight_decay and state_bits == 32 and max_norm is None:
             self.net_opt = DenseAdam(learned, lr=net_lr)
         else:
-            groups = [{'params': learned, 'lr': net_lr}]
-            if sp_W is not None:  # decay would pull all of a point's logits together
+            # decay is for the network's weights: it would pull control points to the world's origin, and a point's logits together
+            groups = [{'params': learned[:-1], 'lr': net_lr}, {'params': [self.ctrl], 'lr': net_lr, 'weight_decay': 0.0, 'name': 'ctrl'}]
+            if sp_W is not None:
                 groups.append({'params': [self.sp_W], 'lr': association_lr, 'weight_decay': 0.0, 'name': 'sp_W'})
             self.net_opt = AdamW(groups, weight_decay=weight_decay, state_bits=state_bits, max_norm=max_norm)
         self.sh_degree = scene.sh_degree
