@@ -8,7 +8,9 @@ Gaussians, Adam on the network and the control points.
 tests can compare its gradients with other formulations.
 
 With neighbour logits `sp_W` [N, M] (LBS_method 'W', network.py:514-515) the association of points to control points is learned too, held
-apart by `balance` times the balance loss of the logits; `weight_decay`, `state_bits` and `max_norm` have the network, the control points
+apart by `balance` times a balance loss. `balance_of` says of what: 'neighbours' is the weights that the warp uses, a softmax over the logits of each
+point's K nearest control points; 'logits' is the softmax over all M, which also moves the logits of control points that are not among a point's
+nearest now (those change as both move), and reads and writes all N M of them in every step. `weight_decay`, `state_bits` and `max_norm` have the network, the control points
 and the logits stepped by `AdamW` instead of plain Adam; the network's weights alone decay.
 
 The network runs on the bf16 copies of its weights that it made when it was first called, since the network's plain optimiser
@@ -23,7 +25,7 @@ import torch
 from torch import Tensor
 
 from fast_sp_gs_amd.adamw import AdamW
-from fast_sp_gs_amd.balance import balance_loss
+from fast_sp_gs_amd.balance import balance_loss, neighbour_balance
 from fast_sp_gs_amd.deform import _FUSED_WARPS, DeformNetwork, _fused_deform, deform_apply, superpoint_deform
 from fast_sp_gs_amd.renderer import GS_2D_render
 from fast_sp_gs_amd.sparse_gaussian_adam import DenseAdam, SparseGaussianAdam
@@ -39,7 +41,8 @@ class DynamicStep:
                  local_frame: bool = True, warp_method: str = 'LBS', LBS_method: str = 'dist', lr: float = 1.6e-4,
                  net_lr: float = 1e-7, lambda_dssim: float = 0.2, background: Optional[Tensor] = None,
                  net: Optional[DeformNetwork] = None, sp_W: Optional[Tensor] = None, association_lr: float = 1e-3,
-                 balance: float = 0.0, weight_decay: float = 0.0, state_bits: int = 32, max_norm: Optional[float] = None):
+                 balance: float = 0.0, weight_decay: float = 0.0, state_bits: int = 32, max_norm: Optional[float] = None,
+                 balance_of: str = 'logits'):
         dev = scene.means3D.device
         self.cam, self.target, self.K, self.temperature = cam, target, K, temperature
         self.warp_method, self.LBS_method, self.lambda_dssim = warp_method, LBS_method, lambda_dssim
@@ -51,6 +54,9 @@ class DynamicStep:
                                       eps=1e-15)
         if (sp_W is None) == (LBS_method == 'W') or (balance and sp_W is None):
             raise ValueError("neighbour logits sp_W go with LBS_method 'W', and a balance with them")
+        if balance_of not in ('logits', 'neighbours'):
+            raise ValueError(f"balance_of must be 'logits' or 'neighbours', got {balance_of!r}")
+        self.balance_of = balance_of
         self.sp_W, self.balance = None if sp_W is None else sp_W.detach().clone().requires_grad_(True), balance
         learned = list(self.net.parameters()) + [self.ctrl]
         if sp_W is None and not weight_decay and state_bits == 32 and max_norm is None:
@@ -79,7 +85,7 @@ class DynamicStep:
                 means3D.detach(), self.ctrl, c_xyz, c_rot, c_scale, c_local, self.K, self.temperature, self.warp_method,
                 self.LBS_method, None, None, columns)
         else:
-            d_xyz, d_rot, d_scale, _, _ = superpoint_deform(
+            d_xyz, d_rot, d_scale, _, indices = superpoint_deform(
                 means3D.detach(), self.ctrl, c_xyz, c_rot, c_scale[:, :columns], sp_rot=c_local, K=self.K,
                 temperature=self.temperature, warp_method=self.warp_method, LBS_method=self.LBS_method, sp_W=self.sp_W)
         xyz, sc, rot = deform_apply(means3D, d_xyz, scales, d_scale, rotations, d_rot)
@@ -88,8 +94,11 @@ class DynamicStep:
                            near=cam.near, far=cam.far, sh_degree=self.sh_degree, sh_features=shs,
                            background=self.background, accum_max_count=self.accum_max_count)
         loss = l1_dssim_loss(out['images'], self.target, self.lambda_dssim)
-        if self.balance:
+        if self.balance and self.balance_of == 'logits':
             loss = loss + self.balance * balance_loss(self.sp_W, 1)[0]
+        elif self.balance:
+            weights = torch.gather(self.sp_W, 1, indices).softmax(-1)  # as the warp forms them, whose own are detached
+            loss = loss + self.balance * neighbour_balance(weights, indices, self.sp_W.shape[1])[0]
         return loss, out
 
     def step(self, t: Tensor):
