@@ -263,8 +263,8 @@ class AdaptiveControl:
                 if state is not None:
                     del opt.state[old]
                     if 'exp_avg' in state:
-                        state['exp_avg'] = torch.zeros_like(new)
-                        state['exp_avg_sq'] = torch.zeros_like(new)
+                        for key in ('exp_avg', 'exp_avg_sq'):  # float32 also of 16-bit parameters, where the optimiser has them so
+                            state[key] = torch.zeros_like(new, dtype=state[key].dtype)
                     elif 'moments8' in state:
                         state['moments8'] = adamw8_state(new)
                     opt.state[new] = state
