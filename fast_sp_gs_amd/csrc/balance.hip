@@ -915,8 +915,8 @@ void launch_rows_backward(int G, int64_t N, int M, int64_t ld, const void* logit
 }
 #undef FSGS_ROW_KERNELS
 
-// The totals' launch has 1024 threads for 16 superpoints, 2^32 of them at most.
-constexpr int kMostSuperpoints = (1 << 26) - 1;
+// The totals' launch has 1024 threads for 16 superpoints, and a launch fewer than 2^32 threads.
+constexpr int kMostSuperpoints = (1 << 26) - 16;
 // Sums of weights have 64 bits, 31 of them below the point.
 constexpr int64_t kMostPairs = ((int64_t) 1 << 33) - 1;
 
