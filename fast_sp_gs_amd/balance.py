@@ -21,7 +21,7 @@ def balance_loss(logits: Tensor, K: int = 1, rows: Optional[Tensor] = None) -> T
     """(loss [], counts [M] int32, importance P [M]) of association logits [N, M] (float32, float16 or bfloat16; sums in float32 or more),
     whose softmax over the superpoints is the weight. Equal logits are chosen by the lowest index; -inf marks a superpoint that a point
     may not use, and is never chosen. `rows` [N] bool: the points that count; the others' logits are not looked at and get a gradient
-    of 0, as do points whose logits are all -inf. K is at most 64, M at most 2^26 - 16, N below 2^31. loss and importance are differentiable in the
+    of 0, as do points whose logits are all -inf. K is at most 64, M at most 2^26 - 16, N below 2^31 - 1. loss and importance are differentiable in the
     logits."""
     return host.balance_loss(logits, K, rows)
 

@@ -928,6 +928,7 @@ bool is_type(int type) { return type == FSGS_DTYPE_F32 || type == FSGS_DTYPE_F16
 using namespace fsgs;
 
 FSGS_API int fsgs_balance_max_choices(void) { return kMostChoices; }
+FSGS_API int fsgs_balance_max_superpoints(void) { return kMostSuperpoints; }
 
 FSGS_API size_t fsgs_balance_loss_workspace_bytes(int64_t N, int M, int dtype) {
   if (N < 0 || M <= 0) return 0;

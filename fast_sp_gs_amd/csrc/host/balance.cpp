@@ -35,6 +35,12 @@ void require_rows(const char* what, const Tensor& rows, const Tensor& like) {
   if (rows.device() != like.device()) fail(std::string(what) + ": all tensors of a call must be on one device");
 }
 
+// Before anything is allocated, which for sizes beyond these takes gigabytes.
+void require_sizes(const char* what, int64_t N, int64_t M) {
+  if (N > INT_MAX - 1) fail(std::string(what) + ": more than 2^31 - 2 points");
+  if (M > fsgs_balance_max_superpoints()) fail(std::string(what) + ": more than " + std::to_string(fsgs_balance_max_superpoints()) + " superpoints");
+}
+
 // A captured backward of a leaf whose accumulation node an eager graph on the default stream keeps alive would have that stream wait for
 // the capture, which ends it and the process: refused while nothing is recorded.
 void refuse_capture_beside_eager(const char* what, const char* name, const Tensor& t) {
@@ -153,7 +159,8 @@ std::tuple<Tensor, Tensor, Tensor> balance_loss(const Tensor& logits, int64_t K,
   refuse_duals(what, logits);
   if (!logits.defined() || !logits.is_cuda() || logits.layout() != at::kStrided) fail("balance_loss: logits must be a CUDA tensor");
   (void) logits_code(logits.scalar_type());
-  if (logits.dim() != 2 || logits.size(1) < 1 || logits.size(1) > INT_MAX) fail("balance_loss: logits must be [N, M] with M >= 1");
+  if (logits.dim() != 2 || logits.size(1) < 1) fail("balance_loss: logits must be [N, M] with M >= 1");
+  require_sizes(what, logits.size(0), logits.size(1));
   const Tensor on = contiguous(opt(rows));
   require_rows(what, on, logits);
   if (K < 1 || K > logits.size(1) || K > fsgs_balance_max_choices())
@@ -178,7 +185,8 @@ std::tuple<Tensor, Tensor, Tensor> neighbour_balance(const Tensor& weights, cons
   require_shape(what, "indices", index, w.sizes());
   if (index.device() != w.device()) fail("neighbour_balance: all tensors of a call must be on one device");
   require_rows(what, on, w);
-  if (M < 1 || M > INT_MAX) fail("neighbour_balance: M must be positive");
+  if (M < 1) fail("neighbour_balance: M must be positive");
+  require_sizes(what, w.size(0), M);
   const c10::DeviceGuard guard(w.device());
   if (at::GradMode::is_enabled() && w.requires_grad()) {
     refuse_capture_beside_eager(what, "weights", weights);

@@ -1030,8 +1030,9 @@ int fsgs_grad_norm_factor(int n_sums, const double* sums, double max_norm, float
  * logits above -inf, the lowest index first (K <= fsgs_balance_max_choices()). rows[N] (optional): 0 leaves a row out, unread. stats[N][2]
  * (optional, 8-byte aligned): what the backward needs of each row. workspace: fsgs_balance_loss_workspace_bytes bytes, 8-byte aligned.
  * The backward writes grad[N, M] (dtype, contiguous) = p (a - sum p a), a = (g_loss M f + g_importance) / T; either of the two upstream
- * gradients (device, g_loss one float, g_importance[M]) may be NULL. N < 2^31, M <= 2^26 - 16. */
+ * gradients (device, g_loss one float, g_importance[M]) may be NULL. N < 2^31 - 1, M <= fsgs_balance_max_superpoints() (2^26 - 16). */
 int fsgs_balance_max_choices(void);
+int fsgs_balance_max_superpoints(void);
 size_t fsgs_balance_loss_workspace_bytes(int64_t N, int M, int dtype);
 int fsgs_balance_loss_forward(int64_t N, int M, int64_t ld, int K, int dtype, const void* logits, const uint8_t* rows,
     float* loss, int32_t* counts, float* importance, int64_t* totals, float* stats, void* workspace, size_t workspace_bytes,
