@@ -607,9 +607,10 @@ __global__ void __launch_bounds__(kWideThreads) balance_wide_backward_kernel(int
 }
 
 // ---- neighbour weights ----------------------------------------------------------------------------------------------------------------
-// Weights lie in [0, 1] (a rounding above 1 is let pass): in units of 2^-31 a block's sums are integers of 64 bits. A weight that is none,
+// Weights lie in [0, 1] (roundings above 1 are let pass, up to kMostWeight): in units of 2^-31 a block's sums are integers of 64 bits. A weight that is none,
 // or an index that is none, is reported and left out.
 constexpr float kWeightUnits = 2147483648.0f;
+constexpr float kMostWeight = 1.0001f;  // its units fit in 32 bits
 
 // A thread takes a row, four neighbours at a time: all loads of four are on their way before the first is looked at. kQuads: K is a
 // multiple of four and the addresses allow 16 bytes. A block keeps the superpoints of one range in LDS (blockIdx.y); beyond kMostRanges of
@@ -655,7 +656,7 @@ __global__ void __launch_bounds__(kNeighbourThreads) balance_neighbours_kernel(i
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
         if (!kQuads && k + d >= K) continue;
-        const bool valid = w[d] >= 0.0f && w[d] <= 1.0001f && (uint64_t) m[d] < (uint64_t) M;
+        const bool valid = w[d] >= 0.0f && w[d] <= kMostWeight && (uint64_t) m[d] < (uint64_t) M;
         if (!valid) {
           invalid = 1;
           continue;

@@ -1039,8 +1039,9 @@ int fsgs_balance_loss_forward(int64_t N, int M, int64_t ld, int K, int dtype, co
     void* stream);
 int fsgs_balance_loss_backward(int64_t N, int M, int64_t ld, int dtype, const void* logits, const float* stats,
     const int32_t* counts, const int64_t* totals, const float* g_loss, const float* g_importance, void* grad, void* stream);
-/* The same of weights[N, K] in [0, 1] with indices[N, K] in [0, M): a row chooses its largest weight, the first of equal ones. A weight or
- * an index outside, in a row that counts, makes loss and importance NaN. The backward's grad[N, K] = a[index], 0 in rows left out. N K < 2^33. */
+/* The same of weights[N, K] in [0, 1] with indices[N, K] in [0, M): a row chooses its largest weight, the first of equal ones. A weight below
+ * 0, above 1.0001 (roundings above 1 pass) or NaN, or an index outside, in a row that counts, makes loss and importance NaN, and the weight or
+ * index counts for nothing. The backward's grad[N, K] = a[index], 0 in rows left out. N K < 2^33. */
 size_t fsgs_neighbour_balance_workspace_bytes(int64_t N, int M);
 int fsgs_neighbour_balance_forward(int64_t N, int M, int K, const float* weights, const int64_t* indices, const uint8_t* rows,
     float* loss, int32_t* counts, float* importance, int64_t* totals, void* workspace, size_t workspace_bytes, void* stream);
