@@ -12,7 +12,9 @@ float16 or bfloat16 tensors on one GPU, of any layout without gaps, fewer than 2
 8-bit moments: the state of a tensor is one uint8 tensor, blocks of 256 consecutive elements under a power of two each; m with sign, 4
 bits of exponent and 3 of fraction, v with 5 and 3. Codes are rounded up or down by a hash of (element, step count, seed) such that
 the mean is the value, since changes of a tenth and a thousandth would never reach the next code otherwise. The moments are formed in
-float64 from the codes, so that a code never hangs on a rounding; equal calls give equal results. An infinity or a NaN in a moment makes
+float64 from the codes; a code's border counts as reached from 2^-44 of the binade (6e-14) below it on, since decimal betas miss borders that 16-bit
+gradients put a moment on. Equal calls give equal results; tensors of a call that have taken as many steps share their random numbers, element by
+element. An infinity or a NaN in a moment makes
 those of its block of 256 NaN.
 """
 from __future__ import annotations

@@ -233,8 +233,9 @@ __device__ __forceinline__ float decoded(uint32_t bits, int exponent) {
   return ldexpf(__builtin_bit_cast(float, bits), exponent + 1 - (1 << kBits));
 }
 // The same the other way round, of a float64, whose upper word has all the bits that count: 3 kept ones and the 16 below them that the noise
-// is added to. What stands below those cannot change the code, so a code is that of the exact value. Betas are decimal numbers: gradients of
-// few bits put moments on a border that the betas' binary neighbours miss by parts in 10^16. A part in 10^13 is added for them.
+// is added to. Betas are decimal numbers: gradients of few bits put moments on a border that the betas' binary neighbours miss by parts
+// in 10^16. A border counts as reached from 256 units in the last place below it on (2^-44 of the binade, 6e-14); farther from it a
+// code is that of the float64 moment.
 constexpr uint64_t kHair = 256;
 template <int kBits>
 __device__ __forceinline__ uint32_t encoded(double x, int exponent, uint32_t noise16, uint32_t least) {
