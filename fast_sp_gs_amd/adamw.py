@@ -7,7 +7,8 @@ largest thing in memory: 8 bytes an element in 32 bits, 2 in 8.
     p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 
 `adamw_step` and `adamw8_step` step lists of tensors, `AdamW` is the optimiser class over them. Parameters and gradients are float32,
-float16 or bfloat16 tensors on one GPU, of any layout without gaps, fewer than 2^34 elements in a call.
+float16 or bfloat16 tensors on one GPU, of any layout without gaps, fewer than 2^34 elements in a call. Tensors that a call writes may not share
+memory with any other of its tensors.
 
 8-bit moments: the state of a tensor is one uint8 tensor, blocks of 256 consecutive elements under a power of two each; m with sign, 4
 bits of exponent and 3 of fraction, v with 5 and 3. Codes are rounded up or down by a hash of (element, step count, seed) such that

@@ -30,15 +30,48 @@ bool alike(const Tensor& a, const Tensor& b) {
          ((a.is_contiguous() && b.is_contiguous()) || (a.strides() == b.strides() && a.is_non_overlapping_and_dense()));
 }
 
-void refuse_twice(const std::string& what, const char* name, const std::vector<Tensor>& list) {
-  std::vector<const void*> at;
-  at.reserve(list.size());
-  bool rising = true;
-  for (const Tensor& t : list)
-    if (t.numel() > 0) rising = rising && (at.empty() || at.back() < t.data_ptr()), at.push_back(t.data_ptr());
-  if (rising) return;
-  std::sort(at.begin(), at.end());
-  if (std::adjacent_find(at.begin(), at.end()) != at.end()) fail(what + ": a " + name + " is there twice");
+struct Written {  // by the call: a tensor for each parameter
+  const char* name;
+  const std::vector<Tensor>& list;
+};
+
+// What a call writes, no other thread of it may read or write: a tensor that is there twice, or views that overlap, would be stepped in a race.
+// Gradients may share their memory among themselves, or be the parameter that they belong to. Lists mostly rise in memory and are merged.
+void refuse_shared(const std::string& what, std::initializer_list<Written> written, const std::vector<Tensor>& params, const std::vector<Tensor>& grads) {
+  struct Range {
+    const char *from, *to, *name;  // name: null for what is only read
+  };
+  const auto before = [](const Range& a, const Range& b) { return a.from < b.from; };
+  std::vector<Range> all;
+  all.reserve((written.size() + 1) * params.size());
+  const auto add = [&](const char* name, const Tensor& t) {
+    const char* from = (const char*) t.const_data_ptr();
+    if (t.numel() > 0) all.push_back({from, from + t.numel() * (int64_t) t.element_size(), name});
+  };
+  const auto merge = [&](size_t from) {
+    if (!std::is_sorted(all.begin() + from, all.end(), before)) std::sort(all.begin() + from, all.end(), before);
+    std::inplace_merge(all.begin(), all.begin() + from, all.end(), before);
+  };
+  for (const Written& w : written) {
+    const size_t from = all.size();
+    for (const Tensor& t : w.list) add(w.name, t);
+    merge(from);
+  }
+  const size_t from = all.size();
+  for (size_t k = 0; k < grads.size(); ++k)
+    if (grads[k].const_data_ptr() != params[k].const_data_ptr()) add(nullptr, grads[k]);
+  merge(from);
+  Range none{nullptr, nullptr, nullptr}, last = none, last_written = none;  // of those so far, the ones that reach farthest
+  for (const Range& r : all) {
+    const Range& other = r.name ? last : last_written;
+    if (r.from < other.to) {
+      if (r.name == other.name && r.from == other.from) fail(what + ": a " + r.name + " is there twice");
+      const auto named = [](const Range& x) { return std::string("a ") + (x.name ? x.name : "gradient"); };
+      fail(what + ": " + named(other) + " and " + named(r) + " share memory");
+    }
+    if (last.to < r.to) last = r;
+    if (r.name && last_written.to < r.to) last_written = r;
+  }
 }
 
 void changed(const Tensor& t) {  // kernels write behind autograd's back: whoever saved or packed the tensor is told
@@ -107,7 +140,6 @@ struct Call {
         if (s.scalar_type() != at::kFloat) fail(w + ": step counts on the device must have dtype torch.float32");
       }
     }
-    refuse_twice(w, "parameter", params), refuse_twice(w, "step count", steps);
     if (has(norm)) {
       require(what, "norm", *norm, at::kFloat), require_device(w, "norm", *norm, device);
       const int64_t room = (int64_t) norm->storage().nbytes() - norm->storage_offset() * 4;
@@ -196,7 +228,7 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
       if (t->scalar_type() != at::kFloat) fail(what + ": moments must have dtype torch.float32, got " + dtype_text(t->scalar_type()));
       if (!alike(*t, params[k])) fail(what + ": tensor " + number(k) + "'s moments differ from it in shape or layout");
     }
-  refuse_twice(what, "moment", m), refuse_twice(what, "moment", v);
+  refuse_shared(what, {{"parameter", params}, {"first moment", m}, {"second moment", v}, {"step count", steps}}, params, call.grads);
   call.advance(steps);
   const float* factor = f32(opt(norm));
   step_all(call, params, steps, set, 0,
@@ -222,7 +254,7 @@ void adamw8_step(const std::vector<Tensor>& params, const std::vector<Tensor>& g
     if (states[k].numel() != adamw8_state_bytes(params[k].numel())) fail(what + ": state " + number(k) + " is that of another number of elements");
     if ((uintptr_t) states[k].data_ptr() % 16) fail(what + ": state " + number(k) + " must lie on a boundary of 16 bytes");
   }
-  refuse_twice(what, "state", states);
+  refuse_shared(what, {{"parameter", params}, {"state", states}, {"step count", steps}}, params, call.grads);
   call.advance(steps);
   const float* factor = f32(opt(norm));
   step_all(call, params, steps, set, (uint32_t) seed,

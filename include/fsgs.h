@@ -992,7 +992,8 @@ int fsgs_adam_masked_update_multi(int n_tensors, int64_t N, const int64_t* M, co
  * one that is being taken), lr, eps, decay and the addresses. dtype (FSGS_DTYPE_F32, _F16, _BF16) is that of param and grad; m and v are
  * float32. norm_and_factor (device, optional): what fsgs_grad_norm_factor wrote; c is 1 without it.
  * rates (device, optional): what fsgs_adamw_rates wrote for the same tensors; step may be NULL then. Addresses need the alignment of
- * their element type; those of four elements are moved in one access. A launch takes fewer than 2^34 elements. */
+ * their element type; those of four elements are moved in one access. A launch takes fewer than 2^34 elements. What it writes must not
+ * overlap anything else that it reads or writes (a parameter may be its own gradient): the host layer checks that, these entries do not. */
 int fsgs_adamw_max_tensors(void);
 int fsgs_adamw_update_multi(int n_tensors, int dtype, const int64_t* count, const double* step, const double* lr, double b1,
     double b2, const double* eps, const double* decay, const void* rates, const float* norm_and_factor, void* const* param,
