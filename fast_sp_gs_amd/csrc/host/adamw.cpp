@@ -138,6 +138,11 @@ struct Call {
       if (device_steps) {
         require_device(w, "step", s, device);
         if (s.scalar_type() != at::kFloat) fail(w + ": step counts on the device must have dtype torch.float32");
+      } else {
+        const auto type = s.scalar_type();  // 16 bits stop at 256 or 2048
+        if (type != at::kFloat && type != at::kDouble && type != at::kInt && type != at::kLong)
+          fail(w + ": step counts must have dtype torch.float32, torch.float64, torch.int32 or torch.int64, got " + dtype_text(type));
+        if (!((type == at::kFloat ? (double) *s.const_data_ptr<float>() : s.item<double>()) >= 0)) fail(w + ": a step count must not be negative");
       }
     }
     if (has(norm)) {
