@@ -20,7 +20,8 @@ int type_code(const std::string& what, const char* name, at::ScalarType type) {
 std::string number(size_t k) { return std::to_string(k); }
 
 void require_device(const std::string& what, const char* name, const Tensor& t, const at::Device& device) {
-  if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided) fail(what + ": " + name + " must be a CUDA tensor");
+  if (t.defined() && t.layout() != at::kStrided) fail(what + ": " + name + " must be dense, sparse tensors are not stepped");
+  if (!t.defined() || !t.is_cuda()) fail(what + ": " + name + " must be a CUDA tensor");
   if (t.device() != device) fail(what + ": all tensors of a call must be on one device");
 }
 
