@@ -114,6 +114,11 @@ class AdamW(torch.optim.Optimizer):
     def __getstate__(self):  # torch keeps the groups and the states alone
         return dict(super().__getstate__(), state_bits=self.state_bits, max_norm=self.max_norm, seed=self.seed, last_norm=None)
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for group in self.param_groups:  # checkpoints from before torch's AdamW had it
+            group.setdefault('capturable', False)
+
     def _state_of(self, p: Tensor, capturable: bool):
         state = self.state[p]
         if not state:
