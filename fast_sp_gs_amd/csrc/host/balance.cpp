@@ -2,8 +2,10 @@
 
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
+#include <torch/csrc/autograd/graph_task.h>
 
 #include <climits>
+#include <unordered_set>
 
 namespace fsgs_host {
 namespace {
@@ -50,6 +52,33 @@ void refuse_capture_beside_eager(const char* what, const char* name, const Tenso
   const auto stream = node->stream();
   if (stream && stream->id() == 0)
     fail(std::string(what) + ": " + name + " is part of an eager graph that is still alive: drop that graph before this call is captured");
+}
+
+// The same for everything that the backward under way has yet to reach: logits made from leaves while an eager graph of those leaves lives, or made
+// eagerly themselves. The engine has the default stream wait for a node's results once the node returns: here is the last place to refuse.
+void refuse_backward_into_eager(const char* what) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  const auto* run = torch::autograd::get_current_graph_task_exec_info();  // empty: all of the graph
+  std::unordered_set<torch::autograd::Node*> seen;
+  std::vector<torch::autograd::Node*> todo{node.get()};
+  while (!todo.empty()) {
+    const auto* at = todo.back();
+    todo.pop_back();
+    for (const auto& edge : at->next_edges()) {
+      auto* next = edge.function.get();
+      if (!next || !seen.insert(next).second) continue;
+      if (run && !run->empty()) {
+        const auto info = run->find(next);
+        if (info == run->end() || !info->second.should_execute()) continue;
+      }
+      const auto stream = next->stream();
+      if (stream && stream->id() == 0)
+        fail(std::string(what) + ": " + next->name() + " is part of an eager graph that is still alive: drop that graph before this call is captured");
+      todo.push_back(next);
+    }
+  }
 }
 
 OptTensor given(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
@@ -105,6 +134,7 @@ struct RowsNode : public torch::autograd::Function<RowsNode> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const char* what = "balance_loss_backward";
+    refuse_backward_into_eager(what);
     const Upstream up(g);
     if (!up.any()) return variable_list(3);
     const auto t = ctx->get_saved_variables();
@@ -134,6 +164,7 @@ struct NeighboursNode : public torch::autograd::Function<NeighboursNode> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const char* what = "neighbour_balance_backward";
+    refuse_backward_into_eager(what);
     const Upstream up(g);
     if (!up.any()) return variable_list(4);
     const auto t = ctx->get_saved_variables();
