@@ -165,11 +165,16 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """Also a checkpoint with moments of the other width. torch casts what it loads to the parameter's type, which moments do not
-        have here: they are taken from the checkpoint itself."""
+        have here: they are taken from the checkpoint itself. 8-bit moments follow the memory: a parameter that takes them over lies as the one
+        that they were kept of."""
         if any(group.get('amsgrad') or group.get('maximize') for group in state_dict['param_groups']):
             raise ValueError('AdamW: checkpoints of amsgrad or maximize steps cannot be taken over')
+        ids = list(chain.from_iterable(group['params'] for group in state_dict['param_groups']))
+        for k, p in zip(ids, chain.from_iterable(group['params'] for group in self.param_groups)):
+            for key, t in (state_dict['state'].get(k) or {}).items():
+                if key in ('exp_avg', 'exp_avg_sq') and t.shape != p.shape or key == 'moments8' and t.numel() != host.adamw8_state_bytes(p.numel()):
+                    raise ValueError(f"AdamW: the checkpoint's {key} has shape {tuple(t.shape)}, which a parameter of {tuple(p.shape)} does not have")
         super().load_state_dict(state_dict)
-        ids = chain.from_iterable(group['params'] for group in state_dict['param_groups'])
         own = [(p, group['capturable']) for group in self.param_groups for p in group['params']]
         for k, (p, capturable) in zip(ids, own):
             saved = state_dict['state'].get(k)
