@@ -10,7 +10,7 @@ tests can compare its gradients with other formulations.
 With neighbour logits `sp_W` [N, M] (LBS_method 'W', network.py:514-515) the association of points to control points is learned too, held
 apart by `balance` times a balance loss. `balance_of` says of what: 'neighbours' is the weights that the warp uses, a softmax over the logits of each
 point's K nearest control points; 'logits' is the softmax over all M, which also moves the logits of control points that are not among a point's
-nearest now (those change as both move), and reads and writes all N M of them in every step. `weight_decay`, `state_bits` and `max_norm` have the network, the control points
+nearest now (those change as both move). `weight_decay`, `state_bits` and `max_norm` have the network, the control points
 and the logits stepped by `AdamW` instead of plain Adam; the network's weights alone decay.
 
 The network runs on the bf16 copies of its weights that it made when it was first called, since the network's plain optimiser
