@@ -290,7 +290,8 @@ __device__ __forceinline__ void exponentials(float x[kVals], float shift) {
 // stay in the registers of the lane that reads it, for all rows of a wavefront. Vector instructions for each row: 127 of 512 float32 with 4
 // chosen (300 000 x 512 105 - 122 us, 5.0 - 5.8 TB/s: memory), 142 of 512 bfloat16 (300 000 x 512 105 us, 2.9 TB/s, 0.9 of the cycles issue),
 // 498 of 2000 bfloat16 with 8 chosen (400 000 x 2000 539 us, 3.0 TB/s, 0.7 of the cycles, three wavefronts a SIMD; one chosen 4.4 TB/s), 22
-// of 64 bfloat16 (200 000 x 64 19 us, of 1M 52 us, 2.4 TB/s, 0.95 of the cycles).
+// of 64 bfloat16 (200 000 x 64 19 us, of 1M 52 us, 2.4 TB/s, 0.95 of the cycles). Rows that do not begin and end with pieces of 16 bytes take three
+// times the loads: 300 000 x 501 161 - 174 us in float32, 158 - 167 in bfloat16.
 template <typename T, int kLanes, int kVals, Access kAccess>
 __global__ void __launch_bounds__(row_threads(kVals), row_waves(kVals)) balance_rows_kernel(int64_t N, int M, int64_t ld, int K,
     const T* __restrict__ logits, const uint8_t* __restrict__ rows, float2* __restrict__ stats, float* __restrict__ sums,
@@ -385,7 +386,8 @@ __global__ void __launch_bounds__(row_threads(kVals), row_waves(kVals)) balance_
 }
 
 // The access also of the gradient's rows. The weights are formed again from the row's shift and scale, 8 bytes a row: reading N M and writing
-// N M is what bounds it. 300 000 x 512 float32 210 - 221 us (5.6 - 5.9 TB/s), 200 000 x 64 bfloat16 with a third of the rows left out 15 us.
+// N M is what bounds it. 300 000 x 512 float32 210 - 221 us (5.6 - 5.9 TB/s), 200 000 x 64 bfloat16 with a third of the rows left out 15 us. Element by
+// element (rows that are not whole pieces) 300 000 x 501 takes 391 us, in bfloat16 334 (119 of 512).
 template <typename T, int kLanes, int kVals, Access kAccess>
 __global__ void __launch_bounds__(256) balance_rows_backward_kernel(int64_t N, int M, int64_t ld, const T* __restrict__ logits,
     const float2* __restrict__ stats, const int* __restrict__ counts, const int64_t* __restrict__ totals,
@@ -464,8 +466,9 @@ __global__ void __launch_bounds__(256) balance_rows_backward_kernel(int64_t N, i
 
 // ---- rows of more superpoints than a wavefront's lanes hold: a block a row ----------------------------------------------------------
 // kPer: values of the row in each thread's registers, its columns' sums and counts beside them; 0: of more than 16 384 superpoints, read
-// again for every step, the sums in memory. Bound by the 2 + 2 K reductions over the block, two barriers each: 20 000 x 5000 in float32, 4 chosen,
-// 431 us forward and 571 with the backward (0.9 and 2.1 TB/s), 1179 and 1484 read again by 256 threads; 2000 x 50 000 1154 and 1457.
+// again for every step, the sums in memory. Most of the time goes to the 2 + 2 K reductions over the block, two barriers each (vector units 0.61 of
+// the busy cycles, the rest waits): 20 000 x 5000 in float32, 4 chosen, 411 - 431 us forward and 551 - 571 with the backward (0.9 and 2.1
+// TB/s), 1179 and 1484 read again by 256 threads; 2000 x 50 000 1154 and 1457.
 constexpr int kWideThreads = 1024, kMostPer = 16;
 template <typename F>
 __device__ __forceinline__ int over_block(int x, int none, F f, int* s) {  // all threads get the result; as over_lanes
