@@ -46,7 +46,7 @@ void refuse_shared(const std::string& what, std::initializer_list<Written> writt
   std::vector<Range> all;
   all.reserve((written.size() + 1) * params.size());
   const auto add = [&](const char* name, const Tensor& t) {
-    const char* from = (const char*) t.const_data_ptr();
+    const char* from = (const char*) (name ? t.data_ptr() : t.const_data_ptr());  // what is written has memory of its own from here on
     if (t.numel() > 0) all.push_back({from, from + t.numel() * (int64_t) t.element_size(), name});
   };
   const auto merge = [&](size_t from) {
