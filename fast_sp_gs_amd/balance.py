@@ -29,5 +29,6 @@ def balance_loss(logits: Tensor, K: int = 1, rows: Optional[Tensor] = None) -> T
 def neighbour_balance(weights: Tensor, indices: Tensor, M: int, rows: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
     """`balance_loss` of neighbour weights [N, K] in [0, 1] with their superpoints' indices [N, K] (what `calc_LBS_weight` returns), of
     M superpoints; chosen is a point's neighbour of largest weight, the first of equal ones. An index may be there twice. A weight that
-    is negative, above 1.0001 (roundings above 1 pass) or NaN, or an index outside [0, M), in a row that counts makes loss and importance NaN. Weights are added in units of 2^-31; N K is below 2^33."""
+    is negative, above 1.0001 (roundings above 1 pass) or NaN, or an index outside [0, M), in a row that counts makes loss and importance
+    NaN. Weights are added in units of 2^-31; N K is below 2^33."""
     return host.neighbour_balance(weights, indices, M, rows)

@@ -203,7 +203,8 @@ __global__ void __launch_bounds__(256) adamw_kernel(AdamwTable t, Step s, const 
 // ---- 8-bit moments ----------------------------------------------------------------------------------------------------------------
 // 16 bytes an element in float32 (10 in 16 bits), the exponents 4 in 256: memory in float32, 171M elements 432 - 447 us (6.1 - 6.3 TB/s). In 16 bits
 // decoding, the step, the hash and encoding take longer than the accesses: 8M in bfloat16 24 us (3.3 TB/s), 21 with ten operations an element
-// less (314 vector instructions for 256 elements; the vector units issue in 0.95 of the busy cycles, with 64M elements in all of them, in float32 0.86). Two blocks for each wavefront were slower.
+// less (314 vector instructions for 256 elements; the vector units issue in 0.95 of the busy cycles, with 64M elements in all of them, in float32
+// in 0.86). Two blocks for each wavefront were slower.
 __host__ __device__ __forceinline__ uint32_t mixed(uint32_t x) {
   x = (x ^ (x >> 16)) * 0xBB67AE85u;
   x = (x ^ (x >> 15)) * 0x3C6EF373u;

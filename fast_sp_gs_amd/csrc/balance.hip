@@ -610,8 +610,8 @@ __global__ void __launch_bounds__(kWideThreads) balance_wide_backward_kernel(int
 }
 
 // ---- neighbour weights ----------------------------------------------------------------------------------------------------------------
-// Weights lie in [0, 1] (roundings above 1 are let pass, up to kMostWeight): in units of 2^-31 a block's sums are integers of 64 bits. A weight that is none,
-// or an index that is none, is reported and left out.
+// Weights lie in [0, 1] (roundings above 1 are let pass, up to kMostWeight): in units of 2^-31 a block's sums are integers of 64 bits. A weight that
+// is none, or an index that is none, is reported and left out.
 constexpr float kWeightUnits = 2147483648.0f;
 constexpr float kMostWeight = 1.0001f;  // its units fit in 32 bits
 

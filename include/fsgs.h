@@ -1000,7 +1000,8 @@ int fsgs_adamw_update_multi(int n_tensors, int dtype, const int64_t* count, cons
     const void* const* grad, float* const* m, float* const* v, void* stream);
 /* The same with both moments in 8 bits: state[q] has fsgs_adamw8_state_bytes(count[q]) bytes, 16-byte aligned, all zero before the first
  * step. Blocks of 256 elements under one exponent per moment; the moments are formed in float64, and their codes rounded by a hash of
- * (element, step, seed) so that they are right on average, a border being reached from 2^-44 of the binade below it on; an infinity or a NaN among a block's moments makes all of the block's NaN. */
+ * (element, step, seed) so that they are right on average, a border being reached from 2^-44 of the binade below it on; an infinity or a NaN
+ * among a block's moments makes all of the block's NaN. */
 size_t fsgs_adamw8_state_bytes(int64_t count);
 int fsgs_adamw8_update_multi(int n_tensors, int dtype, const int64_t* count, const double* step, const double* lr, double b1,
     double b2, const double* eps, const double* decay, uint32_t seed, const void* rates, const float* norm_and_factor,
